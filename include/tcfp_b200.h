@@ -343,6 +343,88 @@ int32_t tcfp_bf16_dw_gemm(const void* x, const void* g_hi, const void* g_lo,
                           void* out, int32_t out_dtype, int64_t tokens,
                           int64_t k_in, int64_t n_out, void* stream);
 
+/* ---- operators that end in 8 bits in front of a linear layer ------------- */
+/*
+ * No counterpart in the reference, whose layer quantizes what the norm or the
+ * activation has written in 16 bits in a pass of its own.
+ *
+ * Each writes rows x width 8-bit codes of an FP32 row y, which it never stores:
+ *   block_size 32/64/128: E4M3 codes (dense), scale_out = int8 exponent plane
+ *       (width/bs, rows) and sf_out (nullable) = packed E8M0 copy, by the rule
+ *       of tcfp_quantize; rows of all tensors 16-byte aligned.  A NaN stays
+ *       NaN, an infinity saturates.
+ *   block_size 0: int8 codes = round_half_even(y / s) with one float
+ *       s = max(max |y|, 1e-12) / 127 for each row, rounded to FP32, in
+ *       scale_out; any alignment and width.  A row that holds a NaN or an
+ *       infinity has a scale that is not finite.
+ * ld_* are row pitches in elements.  ld_codes >= width; what lies between them
+ * is not written.  deq_bf16_out (nullable, dense) receives the values the
+ * codes stand for, rounded to bf16.  1 <= rows < 2^31, width <= 2^26.
+ *
+ * tcfp_add_rms_norm_quantize: h = x + residual rounded to dtype (residual
+ *   nullable: h = x), y = h * rsqrt(mean(h^2) + eps) * weight.  h_out (dense,
+ *   required with a residual) and rstd_out (rows floats) are nullable.  x,
+ *   residual and h_out have type dtype.  width <= 32768.
+ * tcfp_silu_mul_quantize: y = gate * sigmoid(gate) * up.
+ * tcfp_int8_quantize_rows: y = x (block_size 0 only).
+ */
+int32_t tcfp_add_rms_norm_quantize(const void* x, int64_t ld_x,
+                                   const void* residual, int64_t ld_residual,
+                                   int32_t dtype, const void* weight,
+                                   int32_t w_dtype, float eps, void* h_out,
+                                   float* rstd_out, uint8_t* codes,
+                                   int64_t ld_codes, void* scale_out,
+                                   uint8_t* sf_out, void* deq_bf16_out,
+                                   int64_t rows, int64_t width,
+                                   int32_t block_size, void* stream);
+int32_t tcfp_silu_mul_quantize(const void* gate, int64_t ld_gate,
+                               const void* up, int64_t ld_up, int32_t dtype,
+                               uint8_t* codes, int64_t ld_codes,
+                               void* scale_out, uint8_t* sf_out,
+                               void* deq_bf16_out, int64_t rows, int64_t width,
+                               int32_t block_size, void* stream);
+int32_t tcfp_int8_quantize_rows(const void* x, int64_t ld_x, int32_t dtype,
+                                uint8_t* codes, int64_t ld_codes,
+                                float* scale_out, void* deq_bf16_out,
+                                int64_t rows, int64_t width, void* stream);
+/*
+ * Backward of the norm, the rounding to 8 bits taken as the identity:
+ *   g = dy * weight, hat = h * rstd
+ *   dx = rstd * (g - hat * mean(g * hat)) + dh      (dh nullable)
+ *   dw[c] = sum over rows of dy * hat
+ * dx (dense) is the gradient of x and of the residual; dy, h, dh and dx have
+ * type dtype, dw is FP32.  The sums' order depends on the number of rows and
+ * of SMs only: repeated calls return identical bits.  workspace:
+ * tcfp_rms_norm_backward_workspace_bytes(rows, width), 16-byte aligned.
+ */
+size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h,
+                               int64_t ld_h, const float* rstd, int32_t dtype,
+                               const void* weight, int32_t w_dtype,
+                               const void* dh, int64_t ld_dh, void* dx,
+                               float* dw, void* workspace, int64_t rows,
+                               int64_t width, void* stream);
+/* Backward of silu(gate) * up, all of type dtype. */
+int32_t tcfp_silu_mul_backward(const void* dy, int64_t ld_dy, const void* gate,
+                               int64_t ld_gate, const void* up, int64_t ld_up,
+                               int32_t dtype, void* dgate, int64_t ld_dgate,
+                               void* dup, int64_t ld_dup, int64_t rows,
+                               int64_t width, void* stream);
+
+/* ---- int8 product ---------------------------------------------------------- */
+/*
+ * out(M,N) = (sum_k a[m,k] * b[n,k]) * s_a[m] * s_b[n] + bias[n]
+ * with int8 a (M,K), b (N,K) of row pitches ld_a, ld_b bytes (multiples of 16,
+ * bases 16-byte aligned), s_a (M) and s_b (N) floats, bias (nullable, N
+ * floats), out f32|bf16 dense.  The integer sum is exact: K <= 131071.  The
+ * factors are applied in FP32 in the order written.  No counterpart in the
+ * reference.
+ */
+int32_t tcfp_int8_gemm(const int8_t* a, int64_t ld_a, const float* s_a,
+                       const int8_t* b, int64_t ld_b, const float* s_b,
+                       const float* bias, void* out, int32_t out_dtype,
+                       int64_t M, int64_t N, int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

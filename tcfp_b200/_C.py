@@ -8,7 +8,7 @@ the caller gets a ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int32, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 import torch
@@ -60,6 +60,20 @@ _SIGNATURES = {
     "tcfp_bf16_dw_gemm": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p]),
     "tcfp_bf16_dual_gemm": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64,
                                       c_int64, c_int32, c_void_p]),
+    "tcfp_add_rms_norm_quantize": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_float,
+                                             c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+                                             c_int64, c_int32, c_void_p]),
+    "tcfp_silu_mul_quantize": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                         c_void_p, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
+    "tcfp_int8_quantize_rows": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                          c_int64, c_void_p]),
+    "tcfp_rms_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "tcfp_rms_norm_backward": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_void_p, c_int32,
+                                         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "tcfp_silu_mul_backward": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                                         c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
+    "tcfp_int8_gemm": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32,
+                                 c_int64, c_int64, c_int64, c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -25,6 +25,8 @@ UNITS = [
     ("retarget.cu", ["--fmad=false"]),
     ("gemm_sm100.cu", []),
     ("gemm2_sm100.cu", []),
+    ("rowquant.cu", []),
+    ("int8_gemm.cu", []),
     ("noalloc.cu", []),
     ("api.cu", []),
 ]

@@ -481,3 +481,309 @@ def fused_block_scaled_dual_gemm_backward_dx(grad_fp8, w_hi_fp8, w_lo_fp8, grad_
     """Reference name of the dX dispatch (tcfp/kernels.py:2428-2469)."""
     return fused_block_scaled_backward_dx(grad_fp8, w_hi_fp8, w_lo_fp8, grad_scales, w_hi_scales, w_lo_scales,
                                           block_size=block_size)
+
+
+# ---------------------------------------------------------------------------
+# operators that end in 8 bits in front of a linear layer, and the int8 product
+# (no counterpart in the reference, whose layer quantizes a stored 16-bit activation)
+# ---------------------------------------------------------------------------
+
+class QuantizedActivation:
+    """An activation that exists in 8 bits only.
+
+    ``codes`` is ``(rows, width)`` for an activation of ``shape``
+    ``(..., width)``.  ``block_size`` 32/64/128: E4M3 codes and int8 exponent
+    planes ``(width // block_size, rows)`` in ``scales``, what
+    :func:`block_quantize_fp8` returns.  ``block_size`` ``None``: int8 codes
+    and one float scale for each row; the rows start on 16-byte boundaries.
+    ``bf16`` holds the values the codes stand for if they were asked for.
+    ``dtype`` is the type of the tensor the activation was computed from."""
+
+    def __init__(self, codes, scales, block_size, shape, dtype, bf16=None):
+        self.codes, self.scales, self.block_size = codes, scales, block_size
+        self.shape, self.dtype, self.bf16 = torch.Size(shape), dtype, bf16
+        # stands for the activation in the autograd graph (see nn.add_rms_norm); its values are never read
+        self._handle = None
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dequantize(self) -> torch.Tensor:
+        """The values the codes stand for, bf16, in ``shape``."""
+        if self.bf16 is not None:
+            return self.bf16.reshape(self.shape)
+        if self.codes.numel() == 0:
+            return torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
+        if self.block_size is not None:
+            with torch.cuda.device(self.device):
+                return block_dequantize_bf16(self.codes, self.scales, self.block_size).reshape(self.shape)
+        return (self.codes.float() * self.scales[:, None]).to(torch.bfloat16).reshape(self.shape)
+
+
+def _rows_of(t: torch.Tensor, who: str, name: str) -> tuple[torch.Tensor, int]:
+    """``(..., width)`` f32 or bf16 -> ``(rows, width)`` with unit column
+    stride, and the row pitch in elements; a view where the strides allow."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: tcfp_b200 runs on CUDA (sm_100) tensors only, got a {t.device} {name}")
+    _C.dtype_code(t)
+    if t.ndim == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{who}: {name} needs a last dimension of at least 1, got shape {tuple(t.shape)}")
+    t = t.detach()
+    if t.ndim != 2:
+        rows = 1
+        for n in t.shape[:-1]:
+            rows *= n
+        t = t.reshape(rows, t.shape[-1])
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    # the pitch of a single row is never used: give it one that does not stand in the way of wide accesses
+    return t, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 16) * 16
+
+
+def _same(t: torch.Tensor | None, like: torch.Tensor, who: str, name: str, like_name: str) -> None:
+    if t is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{who}: {name} ({tuple(t.shape)}, {t.dtype}, {t.device}) must match {like_name} "
+                         f"({tuple(like.shape)}, {like.dtype}, {like.device})")
+
+
+def _vector(t: torch.Tensor, n: int, device, who: str, name: str, dtypes=(torch.float32,)) -> torch.Tensor:
+    if t.shape != (n,) or t.dtype not in dtypes or t.device != device:
+        raise ValueError(f"{who}: {name} must be a ({n},) tensor of {' or '.join(str(d) for d in dtypes)} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.detach().contiguous()
+
+
+def _launch(device: torch.device, fn, *args) -> None:
+    """Calls a C entry point on ``device``'s current stream."""
+    if device.index == torch.cuda.current_device():
+        _C.check(fn(*args, _C.stream()))
+    else:
+        with torch.cuda.device(device):
+            _C.check(fn(*args, _C.stream()))
+
+
+def _pitch16(t: torch.Tensor, ld: int) -> bool:
+    return t.data_ptr() % 16 == 0 and (ld * t.element_size()) % 16 == 0
+
+
+def _check_block(block_size, width: int, who: str) -> None:
+    if block_size is None:
+        return
+    if block_size not in (32, 64, 128):
+        raise ValueError(f"{who}: block_size must be 32, 64, 128 or None (int8, one scale for each row), got {block_size}")
+    if width % block_size != 0:
+        raise ValueError(f"{who}: width ({width}) must be divisible by block_size ({block_size})")
+
+
+def _alloc_quantized(x: torch.Tensor, rows: int, width: int, block_size, want_bf16: bool, shape) -> tuple:
+    """The outputs of a row quantizer: ``(QuantizedActivation, sf or None)``."""
+    dev = x.device
+    deq = torch.empty((rows, width), dtype=torch.bfloat16, device=dev) if want_bf16 else None
+    if block_size is not None:
+        codes = torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty((width // block_size, rows), dtype=torch.int8, device=dev)
+        sf = _alloc_sf(rows, width, block_size, dev)
+        _attach_sf(scales, sf, block_size)
+    else:
+        # the int8 product reads rows that start on 16-byte boundaries
+        codes = torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=dev)[:, :width]
+        scales = torch.empty(rows, dtype=torch.float32, device=dev)
+        sf = None
+    return QuantizedActivation(codes, scales, block_size, shape, x.dtype, deq), sf
+
+
+def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5, *,
+                          block_size: int | None = None, want_bf16: bool = False):
+    """RMS norm with the residual's addition and an output in 8 bits, one
+    pass: ``h = x + residual`` (rounded to ``x.dtype``), ``y = h *
+    rsqrt(mean(h^2) + eps) * weight`` in FP32, quantized.  Returns
+    ``(QuantizedActivation of y, h, rstd)`` with ``rstd`` ``(rows,)`` FP32;
+    without a residual ``h`` is ``x``.  ``x`` is ``(..., width)`` FP32 or bf16
+    with ``width <= 32768``, ``weight`` ``(width,)`` FP32 or bf16."""
+    who = "add_rms_norm_quantize"
+    x2d, ld_x = _rows_of(x, who, "x")
+    _same(residual, x, who, "residual", "x")
+    rows, width = x2d.shape
+    _check_block(block_size, width, who)
+    if width > 32768:
+        raise ValueError(f"{who}: width ({width}) must be at most 32768")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"{who}: eps must be finite and not negative, got {eps}")
+    w = _vector(weight, width, x.device, who, "weight", (torch.float32, torch.bfloat16))
+    r2d, ld_r = (None, 0) if residual is None else _rows_of(residual, who, "residual")
+    if block_size is not None:
+        if not _pitch16(x2d, ld_x):
+            x2d, ld_x = x2d.clone(memory_format=torch.contiguous_format), width
+        if r2d is not None and not _pitch16(r2d, ld_r):
+            r2d, ld_r = r2d.clone(memory_format=torch.contiguous_format), width
+        if w.data_ptr() % 16:
+            w = w.clone()
+    q, sf = _alloc_quantized(x, rows, width, block_size, want_bf16, x.shape)
+    h = torch.empty((rows, width), dtype=x.dtype, device=x.device) if residual is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows > 0:
+        _launch(x.device, _C.load().tcfp_add_rms_norm_quantize, _C.ptr(x2d), ld_x, _C.ptr(r2d), ld_r, _C.dtype_code(x2d),
+                _C.ptr(w), _C.dtype_code(w), float(eps), _C.ptr(h), _C.ptr(rstd), _C.ptr(q.codes),
+                _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
+    return q, x if h is None else h.reshape(x.shape), rstd
+
+
+def _codes_pitch(codes: torch.Tensor) -> int:
+    return codes.stride(0) if codes.dtype == torch.int8 else codes.shape[1]
+
+
+def add_rms_norm_backward(grad: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor,
+                          grad_h: torch.Tensor | None = None):
+    """Gradients of :func:`add_rms_norm_quantize`, the rounding to 8 bits
+    taken as the identity: ``grad`` is that of the normalised output,
+    ``grad_h`` that of the stream ``h`` (``None``: zero).  Returns ``(dx,
+    dw)``: ``dx`` (``h.dtype``, for ``x`` and the residual alike) and ``dw``
+    ``(width,)`` FP32.  Repeated calls return identical bits."""
+    who = "add_rms_norm_backward"
+    h2d, ld_h = _rows_of(h, who, "h")
+    _same(grad, h, who, "grad", "h")
+    _same(grad_h, h, who, "grad_h", "h")
+    rows, width = h2d.shape
+    if width > 32768:
+        raise ValueError(f"{who}: width ({width}) must be at most 32768")
+    w = _vector(weight, width, h.device, who, "weight", (torch.float32, torch.bfloat16))
+    rstd = _vector(rstd, rows, h.device, who, "rstd")
+    if rows == 0:
+        return torch.empty_like(h), torch.zeros(width, dtype=torch.float32, device=h.device)
+    g2d, ld_g = _rows_of(grad, who, "grad")
+    d2d, ld_d = (None, 0) if grad_h is None else _rows_of(grad_h, who, "grad_h")
+    dx = torch.empty((rows, width), dtype=h.dtype, device=h.device)
+    dw = torch.empty(width, dtype=torch.float32, device=h.device)
+    lib = _C.load()
+    with torch.cuda.device(h.device):     # the workspace goes by the device's number of SMs
+        ws = torch.empty(lib.tcfp_rms_norm_backward_workspace_bytes(rows, width), dtype=torch.uint8, device=h.device)
+    _launch(h.device, lib.tcfp_rms_norm_backward, _C.ptr(g2d), ld_g, _C.ptr(h2d), ld_h, _C.ptr(rstd), _C.dtype_code(h2d),
+            _C.ptr(w), _C.dtype_code(w), _C.ptr(d2d), ld_d, _C.ptr(dx), _C.ptr(dw), _C.ptr(ws), rows, width)
+    return dx.reshape(h.shape), dw
+
+
+def _gate_up(gate: torch.Tensor, up: torch.Tensor | None, who: str):
+    """Row views of gate and up: two tensors, or the halves of one packed ``(..., 2 * width)`` tensor."""
+    if up is None:
+        if gate.ndim == 0 or gate.shape[-1] % 2 != 0:
+            raise ValueError(f"{who}: a packed gate_up needs an even last dimension, got shape {tuple(gate.shape)}")
+        width = gate.shape[-1] // 2
+        both, ld = _rows_of(gate, who, "gate_up")
+        return both[:, :width], ld, both[:, width:], ld, gate.shape[:-1] + (width,)
+    _same(up, gate, who, "up", "gate")
+    g2d, ld_g = _rows_of(gate, who, "gate")
+    u2d, ld_u = _rows_of(up, who, "up")
+    return g2d, ld_g, u2d, ld_u, gate.shape
+
+
+_MAX_ROW = 1 << 26
+
+
+def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor | None = None, *, block_size: int | None = None,
+                      want_bf16: bool = False) -> QuantizedActivation:
+    """``silu(gate) * up`` in FP32, quantized, one pass.  ``up=None``: ``gate``
+    is the packed ``(..., 2 * width)`` output of a fused gate/up projection."""
+    who = "silu_mul_quantize"
+    g2d, ld_g, u2d, ld_u, shape = _gate_up(gate, up, who)
+    rows, width = g2d.shape
+    _check_block(block_size, width, who)
+    if width > _MAX_ROW:
+        raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
+    if block_size is not None:
+        if not _pitch16(g2d, ld_g):
+            g2d, ld_g = g2d.clone(memory_format=torch.contiguous_format), width
+        if not _pitch16(u2d, ld_u):
+            u2d, ld_u = u2d.clone(memory_format=torch.contiguous_format), width
+    q, sf = _alloc_quantized(gate, rows, width, block_size, want_bf16, shape)
+    if rows > 0:
+        _launch(gate.device, _C.load().tcfp_silu_mul_quantize, _C.ptr(g2d), ld_g, _C.ptr(u2d), ld_u, _C.dtype_code(g2d),
+                _C.ptr(q.codes), _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(sf), _C.ptr(q.bf16), rows, width,
+                block_size or 0)
+    return q
+
+
+def silu_mul_backward(grad: torch.Tensor, gate: torch.Tensor, up: torch.Tensor | None = None):
+    """Gradients of :func:`silu_mul_quantize`, the rounding to 8 bits taken as
+    the identity: ``(dgate, dup)``, or one packed tensor where ``gate`` is
+    packed."""
+    who = "silu_mul_backward"
+    g2d, ld_g, u2d, ld_u, shape = _gate_up(gate, up, who)
+    if grad.shape != shape or grad.dtype != gate.dtype or grad.device != gate.device:
+        raise ValueError(f"{who}: grad must be {tuple(shape)} {gate.dtype} on {gate.device}, got {tuple(grad.shape)} "
+                         f"{grad.dtype} on {grad.device}")
+    rows, width = g2d.shape
+    if width > _MAX_ROW:
+        raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
+    d2d, ld_d = _rows_of(grad, who, "grad")
+    if up is None:
+        both = torch.empty((rows, 2 * width), dtype=gate.dtype, device=gate.device)
+        dg, du, ld = both[:, :width], both[:, width:], 2 * width
+    else:
+        dg = torch.empty((rows, width), dtype=gate.dtype, device=gate.device)
+        du, ld = torch.empty_like(dg), width
+    if rows > 0:
+        _launch(gate.device, _C.load().tcfp_silu_mul_backward, _C.ptr(d2d), ld_d, _C.ptr(g2d), ld_g, _C.ptr(u2d), ld_u,
+                _C.dtype_code(g2d), _C.ptr(dg), ld, _C.ptr(du), ld, rows, width)
+    if up is None:
+        return both.reshape(gate.shape)
+    return dg.reshape(shape), du.reshape(shape)
+
+
+def int8_quantize_rows(x: torch.Tensor, *, want_bf16: bool = False) -> QuantizedActivation:
+    """``(..., width)`` FP32 or bf16 -> int8 codes with one FP32 scale for each
+    row, ``s = max(amax, 1e-12) / 127``, ``code = round(x / s)`` (ties to
+    even): a token's scale for an activation, an output channel's for a weight
+    ``(N, K)``."""
+    who = "int8_quantize_rows"
+    x2d, ld = _rows_of(x, who, "x")
+    rows, width = x2d.shape
+    if width > _MAX_ROW:
+        raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
+    q, _ = _alloc_quantized(x, rows, width, None, want_bf16, x.shape)
+    if rows > 0:
+        _launch(x.device, _C.load().tcfp_int8_quantize_rows, _C.ptr(x2d), ld, _C.dtype_code(x2d), _C.ptr(q.codes),
+                _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(q.bf16), rows, width)
+    return q
+
+
+def _int8_operand(t: torch.Tensor, who: str, name: str) -> tuple[torch.Tensor, int]:
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: tcfp_b200 runs on CUDA (sm_100) tensors only, got a {t.device} {name}")
+    if t.dtype != torch.int8 or t.ndim != 2:
+        raise TypeError(f"{who}: {name} must be a 2-D int8 tensor, got {t.ndim}-D {t.dtype}")
+    pitch = -(-t.shape[1] // 16) * 16
+    if t.data_ptr() % 16 or (t.shape[1] > 1 and t.stride(1) != 1) or \
+            (t.shape[0] > 1 and (t.stride(0) % 16 or t.stride(0) < t.shape[1])):
+        held = torch.empty((t.shape[0], pitch), dtype=torch.int8, device=t.device)[:, :t.shape[1]]
+        held.copy_(t)
+        t = held
+    return t, t.stride(0) if t.shape[0] > 1 else pitch
+
+
+def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``(a @ b.T) * a_scale[:, None] * b_scale + bias`` -> ``(M, N)`` for int8
+    ``a (M, K)`` and ``b (N, K)`` with one FP32 scale for each row of either.
+    The integer sum is exact (``K <= 131071``); the scales and the bias are
+    applied in FP32 and the result is rounded once.  Operands whose rows do
+    not start on 16-byte boundaries are copied to such rows first
+    (:func:`int8_quantize_rows` lays its codes out that way)."""
+    who = "int8_matmul"
+    code = _out_code(out_dtype)
+    a, ld_a = _int8_operand(a, who, "a")
+    b, ld_b = _int8_operand(b, who, "b")
+    (M, K), (N, K2) = a.shape, b.shape
+    if K != K2 or a.device != b.device:
+        raise ValueError(f"{who}: a ({M}, {K}) on {a.device} and b ({N}, {K2}) on {b.device} do not fit")
+    if not 1 <= K <= 131071 or N < 1:
+        raise ValueError(f"{who}: K ({K}) must be in [1, 131071] and N ({N}) at least 1")
+    a_scale = _vector(a_scale, M, a.device, who, "a_scale")
+    b_scale = _vector(b_scale, N, a.device, who, "b_scale")
+    if bias is not None:
+        bias = _vector(bias, N, a.device, who, "bias", (torch.float32, torch.bfloat16)).float()
+    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    if M > 0:
+        _launch(a.device, _C.load().tcfp_int8_gemm, _C.ptr(a), ld_a, _C.ptr(a_scale), _C.ptr(b), ld_b, _C.ptr(b_scale),
+                _C.ptr(bias), _C.ptr(out), code, M, N, K)
+    return out
