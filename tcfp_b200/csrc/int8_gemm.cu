@@ -2,61 +2,546 @@
 //
 //   out[m,n] = (sum_k a[m,k] b[n,k]) * s_a[m] * s_b[n] + bias[n]
 //
-// The sum is an exact 32-bit integer; the two scales are constant along k, so they are applied once to the finished sum.
+// The sum is an exact 32-bit integer; the two scales are constant along k, so they are applied once, to the finished
+// sum.  Two kernels on tcgen05.mma kind::i8, both fed by TMA through a ring of 128-byte-wide stages of K:
+//
+//   int8_pair_kernel  prompts: a pair of CTAs (cta_group::2) owns a 256 x 256 output tile, as the FP8 pair kernel does.
+//   int8_few_kernel   few tokens: bound by the weight's bytes, so the weight takes the 128 rows of the MMA and the tokens
+//                     its 16..256 columns, and the CTAs of a cluster split K; the partial sums meet through distributed
+//                     shared memory.  Integer sums do not depend on the split.
+//
+// Every wait is bounded; see sm100_ptx.cuh.
+#include <cuda.h>
+
 #include "common.cuh"
 #include "launch.h"
+#include "sm100_ptx.cuh"
 
 namespace tcfp {
 namespace {
 
+constexpr int kThreads = 192;       // warp 0 TMA, warp 1 MMA and TMEM, warps 2-5 epilogue
+constexpr int kStageK = 128;        // bytes of K in a stage: one swizzle row
+constexpr int kMmaK = 32;
+constexpr int kTile = 16384;        // 128 rows x 128 bytes
+
 struct Int8Params {
-  const int8_t *a, *b;
-  int64_t lda, ldb;
   const float *s_a, *s_b, *bias;
   void* out;
   int M, N, K;
+  int k_stages;
+  int group_m;
+  int out_bf16;
+  unsigned int* status;
 };
 
-constexpr int kTile = 64;
-constexpr int kStep = 64;   // bytes of K staged at a time
+// instruction descriptor of kind::i8: S32 accumulator, both operands signed and K-major
+__device__ __forceinline__ uint32_t i8_idesc(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+template <int CTAS>
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+        : "memory");
+}
 
-// 64 x 64 outputs a block of 256 threads, 4 x 4 a thread, dp4a on words staged in shared memory
+// whether all 128 epilogue threads got through a wait: they go on or leave together, so that none is missing at a barrier
+__device__ __forceinline__ bool epi_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "bar.red.and.pred p, 1, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
+
+__device__ __forceinline__ float scaled(int acc, float s_a, float s_b, float bias) {
+  return fmaf(__int2float_rn(acc) * s_a, s_b, bias);
+}
+
+// ---------------------------------------------------------------------------
+// prompts: CTA pairs, 256 x 256 tiles
+// ---------------------------------------------------------------------------
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * kTile;
+constexpr int kPieceBytes = 16384;            // 128 rows x 128 bytes of staged output
+constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 2 * kPieceBytes + 256;
+
 template <bool OUT_BF16>
-__global__ void __launch_bounds__(256) int8_gemm_kernel(const Int8Params p) {
-  __shared__ int s_a[kTile][kStep / 4 + 1], s_b[kTile][kStep / 4 + 1];
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep / 4; i += 256) {
-      const int r = i / (kStep / 4), c = i % (kStep / 4);
-      uint32_t wa = 0, wb = 0;
-      for (int j = 0; j < 4; ++j) {
-        const int k = k0 + 4 * c + j;
-        if (k < p.K && m0 + r < p.M) wa |= (uint32_t)(uint8_t)p.a[(m0 + r) * p.lda + k] << (8 * j);
-        if (k < p.K && n0 + r < p.N) wb |= (uint32_t)(uint8_t)p.b[(n0 + r) * p.ldb + k] << (8 * j);
-      }
-      s_a[r][c] = (int)wa;
-      s_b[r][c] = (int)wb;
+__global__ void __launch_bounds__(kThreads, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                 const __grid_constant__ CUtensorMap tm_out, const Int8Params p, const int tma_store) {
+  constexpr int kStages = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* staging = smem + kStages * kPairStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * kPieceBytes);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kStages);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * kStages), bar_tempty = smem_u32(bars + 2 * kStages + 2);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + 255) / 256;
+  const int num_tiles = tiles_m * tiles_n;
+  // tiles in groups of group_m rows, down the rows first, so that a wave of pairs shares few columns of b
+  auto coords = [&](int tile, int& mb, int& nb) {
+    const int per_group = p.group_m * tiles_n;
+    const int first = tile / per_group * p.group_m;
+    const int gm = min(tiles_m - first, p.group_m);
+    const int in_group = tile % per_group;
+    mb = first + in_group % gm;
+    nb = in_group / gm;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
     }
-    __syncthreads();
-    for (int c = 0; c < kStep / 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(s_a[tm + 16 * i][c], s_b[tn + 16 * j][c], acc[i][j]);
-    __syncthreads();
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull + 8 * b, 1);
+      mbar_init(bar_tempty + 8 * b, 8);   // one arrival per epilogue warp of both CTAs
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-      if (m >= p.M || n >= p.N) continue;
-      float v = (float)acc[i][j] * p.s_a[m] * p.s_b[n];
-      if (p.bias) v += p.bias[n];
-      const int64_t at = (int64_t)m * p.N + n;
-      if (OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-      else reinterpret_cast<float*>(p.out)[at] = v;
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+    if (tma_store) prefetch_tmap(&tm_out);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_holder), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // both CTAs' barriers exist before anything remote touches them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool live = true;
+      for (int tile = pair; live && tile < num_tiles; tile += num_pairs) {
+        int mb, nb;
+        coords(tile, mb, nb);
+        const int row_a = mb * 256 + (int)rank * 128, row_b = nb * 256 + (int)rank * 128;
+        for (int ks = 0; ks < p.k_stages; ++ks) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status)) { live = false; break; }
+          const uint32_t full_leader = mapa(bar_full + 8 * stage, 0);
+          if (rank == 0) mbar_expect_tx(bar_full + 8 * stage, 2 * kPairStageBytes);
+          const uint32_t sa = smem_u32(smem + stage * kPairStageBytes);
+          tma_load_2d_pair(sa, &tm_a, ks * kStageK, row_a, full_leader);
+          tma_load_2d_pair(sa + kTile, &tm_b, ks * kStageK, row_b, full_leader);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+      }
     }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = i8_idesc(256, 256);
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      bool live = true;
+      for (int tile = pair; live && tile < num_tiles; tile += num_pairs) {
+        if (!mbar_wait(bar_tempty + 8 * buf, buf_phase ^ 1, abort_flag, p.status)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(buf * 256);
+        for (int ks = 0; ks < p.k_stages; ++ks) {
+          if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status)) { live = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kPairStageBytes);
+#pragma unroll
+          for (int j = 0; j < kStageK / kMmaK; ++j)
+            tc_mma_i8<2>(d_tmem, make_desc(sa + j * kMmaK, 16, 1024, 2), make_desc(sa + kTile + j * kMmaK, 16, 1024, 2), idesc,
+                         (ks | j) != 0 ? 1u : 0u);
+          tc_commit_pair(bar_empty + 8 * stage);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+        if (!live) break;
+        tc_commit_pair(bar_tfull + 8 * buf);
+        if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else {
+    // epilogue: both CTAs, 128 rows each, 32 accumulator columns at a time
+    constexpr int kPieceCols = OUT_BF16 ? 64 : 32;       // columns in a 128-byte row of the staging buffer
+    constexpr int kElem = OUT_BF16 ? 2 : 4;
+    const int q = warp & 3;
+    const int r_local = q * 32 + lane;
+    const bool issuer = threadIdx.x == 64;
+    int buf = 0, sbuf = 0, pending = 0;
+    uint32_t buf_phase = 0;
+    for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+      int mb, nb;
+      coords(tile, mb, nb);
+      const int row0 = mb * 256 + (int)rank * 128;
+      const float s_a = row0 + r_local < p.M ? __ldg(p.s_a + row0 + r_local) : 0.f;
+      if (!epi_all(mbar_wait(bar_tfull + 8 * buf, buf_phase, abort_flag, p.status))) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
+#pragma unroll 1
+      for (int g = 0; g < 8; ++g) {
+        uint32_t v[32];
+        tmem_ld32(t_row + g * 32, v);
+        tmem_ld_wait();
+        if (g == 7) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa(bar_tempty + 8 * buf, 0));
+        }
+        const int n0 = nb * 256 + g * 32;
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int n = n0 + i < p.N ? n0 + i : p.N - 1;
+          o[i] = scaled((int)v[i], s_a, __ldg(p.s_b + n), p.bias ? __ldg(p.bias + n) : 0.f);
+        }
+        // a staging buffer may be rewritten once the store issued two pieces ago has read it
+        if (!OUT_BF16 || (g & 1) == 0) {
+          if (issuer && pending >= 2) { bulk_wait_read1(); pending = 1; }
+          epi_bar_sync();
+        }
+        uint8_t* piece = staging + sbuf * kPieceBytes + r_local * 128;
+        if constexpr (!OUT_BF16) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(piece + ((c ^ (r_local & 7)) << 4)) =
+                make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * c + 2 * k], o[8 * c + 2 * k + 1]);
+              w[k] = *reinterpret_cast<uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint4*>(piece + ((((g & 1) * 4 + c) ^ (r_local & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (OUT_BF16 && (g & 1) == 0) continue;
+        const int nst = nb * 256 + (OUT_BF16 ? (g >> 1) : g) * kPieceCols;
+        if (tma_store) {
+          fence_async_smem();
+          epi_bar_sync();
+          if (issuer && nst < p.N && row0 < p.M) {
+            tma_store_2d(&tm_out, smem_u32(staging + sbuf * kPieceBytes), nst, row0);
+            bulk_commit();
+            ++pending;
+          }
+        } else {
+          // rows of out that do not start on 16-byte boundaries: a warp writes a row's piece, neighbouring lanes neighbouring
+          // columns
+          epi_bar_sync();
+          const int rows = min(128, p.M - row0), cols = min(kPieceCols, p.N - nst);
+          for (int r = warp - 2; r < rows; r += 4)
+            for (int c = lane; c < cols; c += 32) {
+              const uint8_t* src = staging + sbuf * kPieceBytes + r * 128 + (((c * kElem >> 4) ^ (r & 7)) << 4) + (c * kElem & 15);
+              const int64_t at = (int64_t)(row0 + r) * p.N + nst + c;
+              if constexpr (OUT_BF16) reinterpret_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+              else reinterpret_cast<uint32_t*>(p.out)[at] = *reinterpret_cast<const uint32_t*>(src);
+            }
+        }
+        sbuf ^= 1;
+      }
+      if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+    }
+    if (issuer) bulk_wait0();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    for (int i = 0; i < 20; ++i) __nanosleep(1000);
+  }
+  cluster_sync_all();   // the peer may still be reading operands / signalling barriers of this CTA
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// few tokens: the weight on the rows of the MMA, K split over the CTAs of a cluster
+// ---------------------------------------------------------------------------
+template <int NT>
+struct Few {
+  static constexpr int kStageBytes = kTile + NT * kStageK;
+  // three CTAs an SM while the tokens are few, so that their loads overlap; then two, then one
+  static constexpr int kStages = NT <= 32 ? 4 : NT <= 128 ? 3 : 4;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+  static constexpr uint32_t kTmemCols = NT < 32 ? 32 : NT;
+  static_assert(kStages * kStageBytes >= NT * 128 * 4, "the partial sums reuse the stages");
+};
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// gridDim = (splits, weight tiles, token tiles), cluster = (splits, 1, 1)
+template <int NT>
+__global__ void __launch_bounds__(kThreads)
+int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Int8Params p) {
+  using F = Few<NT>;
+  constexpr int kStages = F::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * F::kStageBytes);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kStages), bar_done = smem_u32(bars + 2 * kStages);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int n0 = blockIdx.y * 128, t0 = blockIdx.z * NT;
+  const int ks0 = (int)((int64_t)p.k_stages * rank / splits), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_holder), F::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int ks = ks0; ks < ks1; ++ks) {
+        if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status)) break;
+        mbar_expect_tx(bar_full + 8 * stage, F::kStageBytes);
+        const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
+        tma_load_2d(sw, &tm_w, ks * kStageK, n0, bar_full + 8 * stage);
+        tma_load_2d(sw + kTile, &tm_x, ks * kStageK, t0, bar_full + 8 * stage);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = i8_idesc(128, NT);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool live = true;
+      for (int ks = ks0; ks < ks1; ++ks) {
+        if (!mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status)) { live = false; break; }
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
+#pragma unroll
+        for (int j = 0; j < kStageK / kMmaK; ++j)
+          tc_mma_i8<1>(tmem_base, make_desc(sw + j * kMmaK, 16, 1024, 2), make_desc(sw + kTile + j * kMmaK, 16, 1024, 2), idesc,
+                       (ks != ks0 || j != 0) ? 1u : 0u);
+        tc_commit(bar_empty + 8 * stage);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+      if (live) tc_commit(bar_done);
+    }
+    __syncwarp();
+  }
+  const int row = ((warp & 3) << 5) | lane;      // of the weight tile; warps 2-5 cover the four lane quarters of TMEM
+  const int n = n0 + row;
+  const int tokens = min(NT, p.M - t0);
+  int* part = reinterpret_cast<int*>(smem);       // (NT, 128) partial sums, once every load and MMA is done
+  float s_b = 0.f, bias = 0.f;
+  auto put = [&](int t, int acc) {
+    const float v = scaled(acc, __ldg(p.s_a + t0 + t), s_b, bias);
+    const int64_t at = (int64_t)(t0 + t) * p.N + n;
+    if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<float*>(p.out)[at] = v;
+  };
+  bool live = true;
+  if (warp >= 2) {
+    if (n < p.N) {
+      s_b = __ldg(p.s_b + n);
+      if (p.bias) bias = __ldg(p.bias + n);
+    }
+    live = mbar_wait(bar_done, 0, abort_flag, p.status);
+    live = __all_sync(0xFFFFFFFFu, live);
+    if (live) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < tokens; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (c + i >= tokens) break;
+          if (splits > 1) part[(c + i) * 128 + row] = (int)v[i];
+          else if (n < p.N) put(c + i, (int)v[i]);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  if (splits > 1) {
+    // every CTA of the cluster sums and writes its share of the tokens
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && live && n < p.N) {
+      const uint32_t mine = smem_u32(part) + row * 4;
+      for (int t = rank; t < tokens; t += splits) {
+        int acc = 0;
+        for (int r = 0; r < splits; ++r) acc += ld_cluster_s32(mapa(mine + t * 512, r));
+        put(t, acc);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();   // the others may still be reading this CTA's sums
+  }
+  __syncthreads();
+  if (*abort_flag) {       // copies that nobody waited for may still be on their way
+    for (int i = 0; i < 20; ++i) __nanosleep(1000);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, F::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres) != cudaSuccess ||
+        qres != cudaDriverEntryPointSuccess)
+      sym = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(sym);
+  }();
+  return fn;
+}
+
+// (rows, cols) matrix with a row pitch in bytes, read or written in boxes of 128 bytes x box_rows, 128-byte swizzle
+int make_map(CUtensorMap* map, CUtensorMapDataType dt, int elem, const void* ptr, int64_t rows, int64_t cols, int64_t pitch,
+             int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(TCFP_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TCFP_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return TCFP_OK;
+}
+
+// raises a kernel's dynamic shared memory limit, once for each device
+template <typename Kernel>
+int allow_smem(Kernel kern, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(TCFP_ERR_UNSUPPORTED, "device index %d out of range", dev);
+  if (!done[dev]) {
+    CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[dev] = true;
+  }
+  return TCFP_OK;
+}
+
+struct Operands {
+  const int8_t *a, *b;
+  int64_t lda, ldb;
+};
+
+template <bool OUT_BF16>
+int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
+  constexpr int kElem = OUT_BF16 ? 2 : 4;
+  CUtensorMap tm_a, tm_b, tm_out;
+  int rc;
+  if ((rc = make_map(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.a, p.M, p.K, o.lda, 128)) != TCFP_OK) return rc;
+  if ((rc = make_map(&tm_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.b, p.N, p.K, o.ldb, 128)) != TCFP_OK) return rc;
+  const int64_t pitch = (int64_t)p.N * kElem;
+  const int tma_store = pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+  tm_out = tm_a;
+  if (tma_store && (rc = make_map(&tm_out, OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, kElem,
+                                  p.out, p.M, p.N, pitch, 128)) != TCFP_OK)
+    return rc;
+  static bool done[64] = {false};
+  if ((rc = allow_smem(int8_pair_kernel<OUT_BF16>, kPairSmem, done)) != TCFP_OK) return rc;
+  p.group_m = 16;
+  const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  const int max_pairs = gemm_sm_budget() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < max_pairs ? tiles : max_pairs)), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {2, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_pair_kernel<OUT_BF16>, tm_a, tm_b, tm_out, p, tma_store));
+  return TCFP_OK;
+}
+
+template <int NT>
+int launch_few(const Operands& o, const Int8Params& p, int splits, cudaStream_t stream) {
+  CUtensorMap tm_w, tm_x;
+  int rc;
+  if ((rc = make_map(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.b, p.N, p.K, o.ldb, 128)) != TCFP_OK) return rc;
+  if ((rc = make_map(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.a, p.M, p.K, o.lda, NT)) != TCFP_OK) return rc;
+  static bool done[64] = {false};
+  if ((rc = allow_smem(int8_few_kernel<NT>, Few<NT>::kSmem, done)) != TCFP_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + NT - 1) / NT));
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Few<NT>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_few_kernel<NT>, tm_w, tm_x, p));
+  return TCFP_OK;
 }
 
 constexpr int64_t kMaxK = 131071;   // 128 * 128 * K stays below 2^31
@@ -68,20 +553,35 @@ using namespace tcfp;
 
 extern "C" int32_t tcfp_int8_gemm(const int8_t* a, int64_t ld_a, const float* s_a, const int8_t* b, int64_t ld_b,
                                   const float* s_b, const float* bias, void* out, int32_t out_dtype, int64_t M, int64_t N,
-                                  int64_t K, void* stream) {
+                                  int64_t K, void* stream_) {
   const char* what = "tcfp_int8_gemm";
+  cudaStream_t stream = (cudaStream_t)stream_;
   if (!a || !b || !s_a || !s_b || !out) return fail(TCFP_ERR_INVALID, "%s: NULL argument", what);
   if (out_dtype != TCFP_F32 && out_dtype != TCFP_BF16) return fail(TCFP_ERR_INVALID, "%s: out dtype %d", what, out_dtype);
-  if (M < 1 || N < 1 || K < 1 || M > (1 << 30) || N > (1 << 30))
-    return fail(TCFP_ERR_INVALID, "%s: M %lld, N %lld, K %lld", what, (long long)M, (long long)N, (long long)K);
+  if (M < 1 || N < 1 || K < 1) return fail(TCFP_ERR_INVALID, "%s: M %lld, N %lld, K %lld", what, (long long)M, (long long)N, (long long)K);
+  // tile indices in 32 bits, weight tiles in gridDim.y
+  if (M > (1 << 30) || N > 65535 * 128) return fail(TCFP_ERR_UNSUPPORTED, "%s: M %lld, N %lld", what, (long long)M, (long long)N);
   if (K > kMaxK) return fail(TCFP_ERR_UNSUPPORTED, "%s: K %lld above %lld could overflow the integer sum", what, (long long)K, (long long)kMaxK);
   if (ld_a < K || ld_b < K || ld_a % 16 || ld_b % 16 || (reinterpret_cast<uintptr_t>(a) & 15u) || (reinterpret_cast<uintptr_t>(b) & 15u))
     return fail(TCFP_ERR_INVALID, "%s: rows of a and b start on 16-byte boundaries, ld >= K", what);
-  const Int8Params p{a, b, ld_a, ld_b, s_a, s_b, bias, out, (int)M, (int)N, (int)K};
-  if ((M + kTile - 1) / kTile > 65535) return fail(TCFP_ERR_UNSUPPORTED, "%s: M %lld", what, (long long)M);
-  const dim3 grid((unsigned)((N + kTile - 1) / kTile), (unsigned)((M + kTile - 1) / kTile));
-  if (out_dtype == TCFP_BF16) int8_gemm_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else int8_gemm_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  CUDA_TRY(cudaGetLastError());
-  return TCFP_OK;
+  const Operands o{a, b, ld_a, ld_b};
+  Int8Params p{};
+  p.s_a = s_a; p.s_b = s_b; p.bias = bias; p.out = out;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  p.k_stages = (int)((K + kStageK - 1) / kStageK);
+  p.out_bf16 = out_dtype == TCFP_BF16;
+  p.status = device_status_ptr();
+  if (M > 512) return p.out_bf16 ? launch_pair<true>(o, p, stream) : launch_pair<false>(o, p, stream);
+  const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  const int64_t ctas = ((N + 127) / 128) * ((M + nt - 1) / nt);
+  const int64_t room = (int64_t)sm_count() * (nt <= 32 ? 3 : nt <= 128 ? 2 : 1);
+  int splits = 1;
+  while (splits < 8 && 2 * splits * ctas <= room && 4 * splits <= p.k_stages) splits *= 2;
+  switch (nt) {
+    case 16: return launch_few<16>(o, p, splits, stream);
+    case 32: return launch_few<32>(o, p, splits, stream);
+    case 64: return launch_few<64>(o, p, splits, stream);
+    case 128: return launch_few<128>(o, p, splits, stream);
+    default: return launch_few<256>(o, p, splits, stream);
+  }
 }
