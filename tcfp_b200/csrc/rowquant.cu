@@ -9,6 +9,7 @@
 // the rule of tcfp_quantize) or int8 with one float scale for each row.  y stays in 32 bits between the operator
 // and the rounding to 8: nothing is rounded to 16 bits on the way.
 #include "common.cuh"
+#include <type_traits>
 #include "launch.h"
 
 namespace tcfp {
@@ -16,7 +17,6 @@ namespace {
 
 enum { OP_NORM = 0, OP_GATE = 1, OP_COPY = 2 };
 
-constexpr int kMaxWarps = 32;
 constexpr int kMaxNormWidth = 32768;     // a row's values stay in the registers of 1024 threads
 constexpr int kMaxGateWidth = 1 << 26;   // column indices in 32 bits, column blocks in gridDim.y
 
@@ -36,71 +36,79 @@ struct RowParams {
   __nv_bfloat16* deq;     // nullable
   int64_t rows;
   int width;
-  int block;
+  int block, block_shift;
+  float inv_width;
 };
 
 // ---- eight values of a row ----------------------------------------------------
-// VEC: eight neighbours, 16-byte accesses.  Otherwise eight values a whole row of threads apart, so that neighbouring
-// threads still touch neighbouring values.
+// A thread's chunk of a row: VEC eight neighbours, 16-byte accesses; otherwise eight values a whole row of threads apart
+// (`step`), so that neighbouring threads still touch neighbouring values.  `p` points at the chunk's first value, `left`
+// values of the row lie there and behind it (none or less: nothing is touched).
 template <bool BF16>
-__device__ __forceinline__ float load1(const void* base, int64_t i) {
-  if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
-  else return reinterpret_cast<const float*>(base)[i];
-}
-template <bool BF16>
-__device__ __forceinline__ void store1(void* base, int64_t i, float v) {
-  if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
-  else reinterpret_cast<float*>(base)[i] = v;
-}
-
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const void* base, int64_t row_start, int i0, int step, int width) {
-  if constexpr (VEC) {
-    if (i0 >= width) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    } else if constexpr (BF16) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + row_start + i0);
-      const uint32_t wd[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(wd[j] << 16);
-        v[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
-      }
-    } else {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + row_start + i0);
-      const float4 lo = p[0], hi = p[1];
-      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-      v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (i0 + j * step < width) ? load1<BF16>(base, row_start + i0 + j * step) : 0.f;
-  }
-}
+using Elem = typename std::conditional<BF16, __nv_bfloat16, float>::type;
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&p);
 }
 
+// As they come from memory, so that a load ahead holds half the registers where they are bf16.
 template <bool BF16, bool VEC>
-__device__ __forceinline__ void store8(const float (&v)[8], void* base, int64_t row_start, int i0, int step, int width) {
-  if constexpr (VEC) {
-    if (i0 >= width) return;
-    if constexpr (BF16) {
-      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(base) + row_start + i0) =
-          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+struct Raw {
+  uint32_t w[BF16 && VEC ? 4 : 8];
+
+  __device__ __forceinline__ void load(const Elem<BF16>* p, int left, int step) {
+    if constexpr (VEC) {
+      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+      if (left > 0) {
+        lo = reinterpret_cast<const uint4*>(p)[0];
+        if constexpr (!BF16) hi = reinterpret_cast<const uint4*>(p)[1];
+      }
+      w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w;
+      if constexpr (!BF16) { w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w; }
     } else {
-      float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + row_start + i0);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i0 + j * step < width) store1<BF16>(base, row_start + i0 + j * step, v[j]);
+      for (int j = 0; j < 8; ++j) w[j] = j * step < left ? __float_as_uint((float)p[j * step]) : 0u;
+    }
   }
+  __device__ __forceinline__ void store(Elem<BF16>* p, int left, int step) const {
+    if constexpr (VEC) {
+      if (left <= 0) return;
+      reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (!BF16) reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j * step < left) p[j * step] = (Elem<BF16>)__uint_as_float(w[j]);
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (BF16 && VEC) return __uint_as_float((j & 1) ? (w[j >> 1] & 0xFFFF0000u) : (w[j >> 1] << 16));
+    else return __uint_as_float(w[j]);
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    if constexpr (BF16 && VEC) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[j]);
+    }
+  }
+};
+
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void load8(float (&v)[8], const void* base, int64_t at, int left, int step) {
+  Raw<BF16, VEC> r;
+  r.load(reinterpret_cast<const Elem<BF16>*>(base) + at, left, step);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = r.get(j);
+}
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void store8(const float (&v)[8], void* base, int64_t at, int left, int step) {
+  Raw<BF16, VEC> r;
+  r.set(v);
+  r.store(reinterpret_cast<Elem<BF16>*>(base) + at, left, step);
 }
 
 // ---- reductions over the threads of one row --------------------------------------
@@ -110,37 +118,37 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// over the 32 or 16 lanes that share a row
 template <bool MAX>
 __device__ __forceinline__ float warp_reduce(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
+    if (o == 16 && blockDim.x < 32) continue;
     const float other = __shfl_xor_sync(0xFFFFFFFFu, v, o);
     v = MAX ? max_nan(v, other) : v + other;
   }
   return v;
 }
-// blockDim.x threads (a multiple of 32) share a row; slots: kMaxWarps floats of shared memory for each row of the block,
-// not used for anything else in the meantime.  The order is fixed.
+// Slots for the warps' parts of the rows side by side in a block.  Two sets, taken in turn: a warp may write the next
+// row's while a slower one reads this row's.
+struct Slots {
+  float v[2][64];
+};
+// blockDim.x threads (16 or a multiple of 32) share a row.  Up to 8 warps: everybody adds up the row's 8 slots (those of absent
+// warps hold 0); more warps have the block to themselves and join by shuffles.  The order is fixed.
 template <bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* slots) {
   v = warp_reduce<MAX>(v);
   const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  float* s = slots + threadIdx.y * warps;
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  if (warps <= 1) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* s = slots + threadIdx.y * 8;
+  if (lane == 0) s[warp] = v;
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  return warp_reduce<MAX>(lane < warps ? s[lane] : 0.f);
-}
-
-// ---- int8 with one scale for each row ----------------------------------------------
-// code = round_half_even(y / s) with the quotient rounded to 32 bits.  y * (1/s) is off by less than 3e-5 of a step, so
-// the division itself is only needed where the product falls that near to the middle between two codes.
-__device__ __forceinline__ int int8_code(float y, float s, float inv_s) {
-  const float q = y * inv_s;
-  float r = rintf(q);
-  if (fabsf(fabsf(q - r) - 0.5f) < 1e-4f) r = rintf(__fdiv_rn(y, s));
-  return __float2int_rn(r);
+  if (warps > 8) return warp_reduce<MAX>(lane < warps ? s[lane] : 0.f);
+  const float4 a = *reinterpret_cast<const float4*>(s), b = *reinterpret_cast<const float4*>(s + 4);
+  if constexpr (MAX) return max_nan(max_nan(max_nan(a.x, a.y), max_nan(a.z, a.w)), max_nan(max_nan(b.x, b.y), max_nan(b.z, b.w)));
+  else return ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
 }
 
 // ---- the operators ------------------------------------------------------------------
@@ -148,160 +156,248 @@ __device__ __forceinline__ int int8_code(float y, float s, float inv_s) {
 // limits 0 and g for large |g|); the result is rounded to 8 bits.
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-// the value in front of the row statistics: the stream h, the gated activation, or x itself
+// eight values of the one or two inputs of a row
 template <int OP, bool BF16, bool VEC>
-__device__ __forceinline__ void load_value(float (&v)[8], const RowParams& p, int64_t row, int i0, int step) {
-  load8<BF16, VEC>(v, p.a, row * p.lda, i0, step, p.width);
-  if constexpr (OP != OP_COPY) {
-    if (OP == OP_NORM && p.b == nullptr) return;
-    float o[8];
-    load8<BF16, VEC>(o, p.b, row * p.ldb, i0, step, p.width);
+struct Inputs {
+  Raw<BF16, VEC> a, b;
+
+  __device__ __forceinline__ void load(const Elem<BF16>* pa, const Elem<BF16>* pb, int left, int step) {
+    a.load(pa, left, step);
+    if (OP == OP_GATE || (OP == OP_NORM && pb != nullptr)) b.load(pb, left, step);
+  }
+  // OP_NORM: a becomes the stream x + residual as it is kept, in the inputs' type; the statistics are those of what is
+  // kept.  The sum is rounded to 32 bits and then to the type, as torch adds.
+  __device__ __forceinline__ void add() {
+    float h[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (OP == OP_GATE) {
-        v[j] = gated(v[j], o[j]);
-      } else {
-        // the stream is kept in the inputs' type and the statistics are those of what is kept
-        v[j] = v[j] + o[j];
-        if constexpr (BF16) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
-      }
+      h[j] = a.get(j) + b.get(j);
+      if constexpr (BF16 && !VEC) h[j] = __bfloat162float(__float2bfloat16_rn(h[j]));
     }
+    a.set(h);
   }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void apply_weight(float (&v)[8], const RowParams& p, float rstd, int i0, int step) {
-  float w[8];
-  if (p.w_bf16) load8<true, VEC>(w, p.w, 0, i0, step, p.width);
-  else load8<false, VEC>(w, p.w, 0, i0, step, p.width);
+  // the value in front of the row statistics: the stream, the gated activation, or x itself
+  __device__ __forceinline__ void value(float (&v)[8]) const {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * w[j];
-}
+    for (int j = 0; j < 8; ++j) v[j] = OP == OP_GATE ? gated(a.get(j), b.get(j)) : a.get(j);
+  }
+};
 
+// ---- int8 with one scale for each row ----------------------------------------------
+// code = round_half_even(y / s) with the quotient rounded to 32 bits.  y * (1/s) is off by less than 3e-5 of a step, so
+// the division itself is only needed where the product falls that near to the middle between two codes.  Adding 1.5 * 2^23
+// rounds half to even and leaves the code in the low byte.
 template <bool VEC>
-__device__ __forceinline__ void store_int8(const float (&v)[8], const RowParams& p, int64_t row, int i0, int step, float s,
+__device__ __forceinline__ void store_int8(const float (&v)[8], uint8_t* codes, __nv_bfloat16* deq, int left, int step, float s,
                                            float inv_s) {
-  int c[8];
+  constexpr float kMagic = 12582912.f;
+  float q[8];
+  float off = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) c[j] = int8_code(v[j], s, inv_s);
+  for (int j = 0; j < 8; ++j) {
+    const float x = v[j] * inv_s;
+    q[j] = x + kMagic;
+    off = fmaxf(off, fabsf(x - (q[j] - kMagic)));
+  }
+  if (off > 0.4999f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], s) + kMagic;
+  }
   if constexpr (VEC) {
-    if (i0 < p.width) {
+    if (left > 0) {
       uint32_t wd[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        wd[k] = (uint32_t)(c[4 * k] & 0xFF) | ((uint32_t)(c[4 * k + 1] & 0xFF) << 8) |
-                ((uint32_t)(c[4 * k + 2] & 0xFF) << 16) | ((uint32_t)c[4 * k + 3] << 24);
-      *reinterpret_cast<uint2*>(p.codes + row * p.ldc + i0) = make_uint2(wd[0], wd[1]);
+        wd[k] = __byte_perm(__byte_perm(__float_as_uint(q[4 * k]), __float_as_uint(q[4 * k + 1]), 0x0040),
+                            __byte_perm(__float_as_uint(q[4 * k + 2]), __float_as_uint(q[4 * k + 3]), 0x0040), 0x5410);
+      *reinterpret_cast<uint2*>(codes) = make_uint2(wd[0], wd[1]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (i0 + j * step < p.width) p.codes[row * p.ldc + i0 + j * step] = (uint8_t)c[j];
+      if (j * step < left) codes[j * step] = (uint8_t)(__float_as_uint(q[j]) & 0xFFu);
   }
-  if (p.deq != nullptr) {
-    float d[8];
+  if (deq != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] = (float)c[j] * s;
-    store8<true, VEC>(d, p.deq, row * (int64_t)p.width, i0, step, p.width);
+    for (int j = 0; j < 8; ++j) q[j] = (q[j] - kMagic) * s;
+    store8<true, VEC>(q, deq, 0, left, step);
   }
 }
 
-// E4M3 codes of eight neighbours; block / 8 neighbouring lanes share an exponent
-__device__ __forceinline__ void store_block(const float (&v)[8], const RowParams& p, int64_t row, int i0, bool live) {
+// E4M3 codes of eight neighbours; block / 8 neighbouring lanes share an exponent.  Returns it.
+__device__ __forceinline__ int store_block(const float (&v)[8], uint8_t* codes, __nv_bfloat16* deq, int left, int block) {
   float am = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) am = fmaxf(am, fabsf(v[j]));
-  const int group = p.block >> 3;
-  for (int o = 1; o < group; o <<= 1) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, o));
-  if (!live || i0 >= p.width) return;
+  am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 1));
+  am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 2));
+  if (block >= 64) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 4));
+  if (block == 128) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 8));
   const int e = block_exponent_fast<false>(am);
-  const float fwd = exp2_int(-e), inv = exp2_int(e);
+  // -126 <= e <= 120: both powers are normal numbers
+  const float fwd = __uint_as_float((uint32_t)(127 - e) << 23), inv = __uint_as_float((uint32_t)(127 + e) << 23);
   uint32_t pc[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) pc[j] = encode_fp8x2<false>(v[2 * j] * fwd, v[2 * j + 1] * fwd);
-  *reinterpret_cast<uint2*>(p.codes + row * p.ldc + i0) = make_uint2(pc[0] | (pc[1] << 16), pc[2] | (pc[3] << 16));
-  if (p.deq != nullptr) {
-    uint32_t d[4];
+  if (left > 0) {
+    *reinterpret_cast<uint2*>(codes) = make_uint2(pc[0] | (pc[1] << 16), pc[2] | (pc[3] << 16));
+    if (deq != nullptr) {
+      uint32_t d[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = decode_fp8x2<false>(pc[j]);
-      d[j] = pack_bf16(f.x * inv, f.y * inv);
-    }
-    *reinterpret_cast<uint4*>(p.deq + row * (int64_t)p.width + i0) = make_uint4(d[0], d[1], d[2], d[3]);
-  }
-  if (i0 % p.block == 0) {
-    const int64_t num_kb = p.width / p.block, kb = i0 / p.block;
-    reinterpret_cast<int8_t*>(p.scale)[kb * p.rows + row] = (int8_t)e;
-    if (p.sf != nullptr) {
-      const int64_t k_groups = (num_kb + 3) >> 2;
-      p.sf[sf_chunk_offset(row, kb, k_groups)] = e8m0_from_exp(e);
-      // the last chunk is filled up with 2^0
-      if (kb == num_kb - 1)
-        for (int64_t k = num_kb; k < 4 * k_groups; ++k) p.sf[sf_chunk_offset(row, k, k_groups)] = 127;
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = decode_fp8x2<false>(pc[j]);
+        d[j] = pack_bf16(f.x * inv, f.y * inv);
+      }
+      *reinterpret_cast<uint4*>(deq) = make_uint4(d[0], d[1], d[2], d[3]);
     }
   }
+  return e;
 }
 
-// blockDim = (threads of a row, rows of the block).  A thread holds 8 * NC values of its row in registers; NC = 0 walks
-// a row of any width and loads it again for each pass.  gridDim.y > 1 (only where no statistic spans the row) splits the
-// row's columns.
-template <int OP, bool BF16, bool VEC, bool BLOCK, int NC>
-__global__ void __launch_bounds__(NC == 1 || NC == 2 ? 512 : 1024) row_quant_kernel(const RowParams p) {
-  __shared__ float s_sum[kMaxWarps], s_max[kMaxWarps];
-  const int T = blockDim.x;
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool live = row < p.rows;
-  const int64_t r = live ? row : p.rows - 1;
-  const int step = T;
-  const int span = 8 * T;
-  const int first = (VEC ? 8 : 1) * (int)threadIdx.x + (NC ? NC : 1) * span * (int)blockIdx.y;
-  const int chunks = NC ? NC : (p.width + span - 1) / span;
-  float v[NC ? NC : 1][8];
+// the exponents of `rows` rows from row0 and of the blocks [kb0, kb0 + blocks), staged as s_e[block][row], to their
+// planes and the packed chunks: runs of the row index, words of four blocks
+__device__ __forceinline__ void flush_exponents(const int8_t* s_e, const RowParams& p, int64_t row0, int rows, int pitch,
+                                                int kb0, int blocks) {
+  const int num_kb = p.width / p.block;
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  blocks = min(blocks, num_kb - kb0);
+  int8_t* plane = reinterpret_cast<int8_t*>(p.scale);
+  // 2^k threads a block of columns, so that runs of rows go to neighbouring threads
+  const int run = rows > 16 ? 32 : rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows;
+  for (int r = tid % run; r < rows; r += run)
+    for (int kb = tid / run; kb < blocks; kb += threads / run)
+      plane[(int64_t)(kb0 + kb) * p.rows + row0 + r] = s_e[kb * pitch + r];
+  if (p.sf == nullptr) return;
+  // kb0 is a multiple of four
+  const int64_t k_groups = (num_kb + 3) >> 2;
+  const int groups = (blocks + 3) >> 2;
+  for (int r = tid % run; r < rows; r += run)
+    for (int g = tid / run; g < groups; g += threads / run) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int kb = 4 * g + j;
+        word |= (uint32_t)(kb < blocks ? e8m0_from_exp(s_e[kb * pitch + r]) : (uint8_t)127) << (8 * j);   // filled up with 2^0
+      }
+      *reinterpret_cast<uint32_t*>(p.sf + sf_chunk_offset(row0 + r, kb0 + 4 * g, k_groups)) = word;
+    }
+}
 
-  float rstd = 1.f;
-  if constexpr (OP == OP_NORM) {
-    float sum = 0.f;
+// blockDim = (threads of a row, rows side by side).  A thread holds 8 * NC values of its row in registers, and while it
+// works on them the inputs of its next row are on their way (NC 1 and 2).  The block walks `turns` rows for each of its
+// blockDim.y places.  gridDim.y > 1 (only where no statistic spans the row) splits the row's columns.  NC = 0 walks a
+// row of any width and loads it again for each pass.
+template <int OP, bool BF16, bool VEC, bool BLOCK, int NC>
+__global__ void __launch_bounds__(NC == 1 ? 256 : NC == 2 ? 512 : 1024, NC == 1 ? 6 : NC == 2 ? 2 : 1)
+row_quant_kernel(const RowParams p, const int turns) {
+  __shared__ __align__(16) Slots s_sum, s_max;
+  extern __shared__ int8_t s_e[];
+  using E = Elem<BF16>;
+  constexpr int kHeld = NC ? NC : 1;
+  constexpr bool AHEAD = NC == 1 || NC == 2;
+  const int step = blockDim.x, span = 8 * step, side = blockDim.y;
+  const int col0 = kHeld * span * (int)blockIdx.y;
+  const int first = (VEC ? 8 : 1) * (int)threadIdx.x + col0;
+  const int chunks = NC ? NC : (p.width + span - 1) / span;
+  const int block_rows = turns * side;
+  const int64_t row0 = (int64_t)blockIdx.x * block_rows;
+  const int64_t below = p.rows - row0;
+  const int places = below < block_rows ? (int)below : block_rows;
+  const E* a = reinterpret_cast<const E*>(p.a) + row0 * p.lda + first;
+  const E* b = OP == OP_COPY || p.b == nullptr ? nullptr : reinterpret_cast<const E*>(p.b) + row0 * p.ldb + first;
+
+  float v[kHeld][8];
+  Inputs<OP, BF16, VEC> in[kHeld];
+  // a place behind the last row loads that row once more and stores nothing
+  auto load_row = [&](int place) {
+    place = min(place, places - 1);
 #pragma unroll
-    for (int c = 0; c < chunks; ++c) {
-      float (&x)[8] = v[NC ? c : 0];
-      load_value<OP, BF16, VEC>(x, p, r, first + c * span, step);
-      if (live && p.h != nullptr) store8<BF16, VEC>(x, p.h, r * (int64_t)p.width, first + c * span, step, p.width);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-    }
-    sum = row_reduce<false>(sum, s_sum);
-    rstd = rsqrtf(sum / (float)p.width + p.eps);
-    if (live && p.rstd != nullptr && threadIdx.x == 0) p.rstd[r] = rstd;
-  }
-  // from here on the values that are rounded to 8 bits
-  auto value = [&](int c) {
-    float (&x)[8] = v[NC ? c : 0];
-    if (OP != OP_NORM || NC == 0) load_value<OP, BF16, VEC>(x, p, r, first + c * span, step);
-    if constexpr (OP == OP_NORM) apply_weight<VEC>(x, p, rstd, first + c * span, step);
+    for (int c = 0; c < kHeld; ++c)
+      in[c].load(a + place * p.lda + c * span, b != nullptr ? b + place * p.ldb + c * span : nullptr, p.width - first - c * span, step);
   };
+  if constexpr (AHEAD) load_row(threadIdx.y);
+  if (step > 32) {      // absent warps' slots; ordered before the first read by the barrier in row_reduce
+    const int tid = threadIdx.y * step + threadIdx.x;
+    if (tid < 64 && (tid & 7) >= (step >> 5)) s_sum.v[0][tid] = s_sum.v[1][tid] = s_max.v[0][tid] = s_max.v[1][tid] = 0.f;
+  }
+
+  for (int turn = 0; turn * side < places; ++turn) {
+    const int place = turn * side + (int)threadIdx.y;
+    const bool live = place < places;
+    const int64_t row = row0 + place;
+    if constexpr (NC != 0) {
+      if constexpr (!AHEAD) load_row(place);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (OP == OP_NORM) {
+          if (b != nullptr) in[c].add();
+          if (live && p.h != nullptr)
+            in[c].a.store(reinterpret_cast<E*>(p.h) + row * p.width + first + c * span, p.width - first - c * span, step);
+        }
+        in[c].value(v[c]);
+      }
+      if constexpr (AHEAD)
+        if (turn + 1 < turns) load_row(place + side);
+    }
+    auto again = [&](int c) {      // NC = 0: chunk c once more
+      const int at = min(place, places - 1);
+      in[0].load(a + at * p.lda + c * span, b != nullptr ? b + at * p.ldb + c * span : nullptr, p.width - first - c * span, step);
+      in[0].value(v[0]);
+    };
+    if constexpr (OP == OP_NORM) {
+      static_assert(NC != 0, "the norm's row stays in registers");
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[c][j], v[c][j], sum);
+      sum = row_reduce<false>(sum, s_sum.v[turn & 1]);
+      const float rstd = rsqrtf(fmaf(sum, p.inv_width, p.eps));
+      if (live && p.rstd != nullptr && threadIdx.x == 0) p.rstd[row] = rstd;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float w[8];
+        if (p.w_bf16) load8<true, VEC>(w, p.w, first + c * span, p.width - first - c * span, step);
+        else load8<false, VEC>(w, p.w, first + c * span, p.width - first - c * span, step);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = v[c][j] * rstd * w[j];
+      }
+    }
+    uint8_t* codes = p.codes + row * p.ldc + first;
+    __nv_bfloat16* deq = p.deq != nullptr ? p.deq + row * p.width + first : nullptr;
+    if constexpr (BLOCK) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int i0 = first - col0 + c * span;
+        const int e = store_block(v[c], codes + c * span, deq != nullptr ? deq + c * span : nullptr,
+                                  live ? p.width - first - c * span : 0, p.block);
+        if (live && (i0 & (p.block - 1)) == 0) s_e[(i0 >> p.block_shift) * block_rows + place] = (int8_t)e;
+      }
+    } else {
+      float am = 0.f;
+#pragma unroll
+      for (int c = 0; c < chunks; ++c) {
+        if constexpr (NC == 0) again(c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) am = max_nan(am, fabsf(v[NC ? c : 0][j]));
+      }
+      am = row_reduce<true>(am, s_max.v[turn & 1]);
+      // a row that holds a NaN or an infinity has no scale
+      const float s = am <= 3.4028235e38f ? __fdiv_rn(fmaxf(am, kAmaxFloor), 127.f) : __uint_as_float(0x7FC00000u);
+      const float inv_s = __frcp_rn(s);
+      if (live && threadIdx.x == 0) reinterpret_cast<float*>(p.scale)[row] = s;
+#pragma unroll
+      for (int c = 0; c < chunks; ++c) {
+        if constexpr (NC == 0) again(c);
+        if (live)
+          store_int8<VEC>(v[NC ? c : 0], codes + c * span, deq != nullptr ? deq + c * span : nullptr, p.width - first - c * span,
+                          step, s, inv_s);
+      }
+    }
+  }
   if constexpr (BLOCK) {
-#pragma unroll
-    for (int c = 0; c < chunks; ++c) {
-      value(c);
-      store_block(v[NC ? c : 0], p, r, first + c * span, live);
-    }
-  } else {
-    float am = 0.f;
-#pragma unroll
-    for (int c = 0; c < chunks; ++c) {
-      value(c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) am = max_nan(am, fabsf(v[NC ? c : 0][j]));
-    }
-    am = row_reduce<true>(am, s_max);
-    const float s = __fdiv_rn(am < kAmaxFloor ? kAmaxFloor : am, 127.f);
-    const float inv_s = __frcp_rn(s);
-    if (live && threadIdx.x == 0) reinterpret_cast<float*>(p.scale)[r] = s;
-#pragma unroll
-    for (int c = 0; c < chunks; ++c) {
-      if constexpr (NC == 0) value(c);
-      if (live) store_int8<VEC>(v[NC ? c : 0], p, r, first + c * span, step, s, inv_s);
-    }
+    __syncthreads();
+    flush_exponents(s_e, p, row0, places, block_rows, col0 >> p.block_shift, kHeld * span >> p.block_shift);
   }
 }
 
@@ -316,76 +412,138 @@ struct NormBwdParams {
   float* dw;                    // (gridDim.x, width) partial sums
   int64_t rows;
   int width;
+  float inv_width;
 };
 
 // dx = rstd * (g - hat * mean(g * hat)) + dh with g = dy * w, hat = h * rstd;  dw = sum over rows of dy * hat.
-// A block walks the rows blockIdx.x, blockIdx.x + gridDim.x, ...; a thread owns the same 8 * NC columns of all of
-// them and keeps their part of dw in registers.
-template <bool BF16, bool VEC, int NC>
+// Bound by memory: 6 bytes in and 2 out a bf16 value.  blockDim = (threads of a row, rows side by side); a block walks
+// every gridDim.x-th group of rows, a thread owns the same 8 columns of all its rows, keeps the weight and its part of dw
+// in registers and has the next row on its way while it works on this one.  32768 x 4096 bf16 180 us (5.96 TB/s, the column
+// sums included); without the row ahead 249 us.
+template <bool BF16, bool VEC>
 __global__ void __launch_bounds__(1024) rms_norm_backward_kernel(const NormBwdParams p) {
-  __shared__ float slots[2][kMaxWarps];
+  __shared__ __align__(16) Slots slots;
+  extern __shared__ float s_acc[];       // (rows side by side, 8, threads of a row)
+  using E = Elem<BF16>;
+  const int step = blockDim.x, side = blockDim.y;
+  const int i0 = (VEC ? 8 : 1) * (int)threadIdx.x, left = p.width - i0;
+  const int tid = threadIdx.y * step + threadIdx.x;
+  if (tid < 64) slots.v[0][tid] = slots.v[1][tid] = 0.f;
+  __syncthreads();
+  float w[8], acc[8];
+  if (p.w_bf16) load8<true, VEC>(w, p.w, i0, left, step);
+  else load8<false, VEC>(w, p.w, i0, left, step);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+
+  Raw<BF16, VEC> dy, h, dh;
+  float rstd;
+  // a row behind the last one is taken as zeros: it adds nothing
+  auto load = [&](int64_t row) {
+    const int n = row < p.rows ? left : 0;
+    dy.load(reinterpret_cast<const E*>(p.dy) + row * p.ld_dy + i0, n, step);
+    h.load(reinterpret_cast<const E*>(p.h) + row * p.ld_h + i0, n, step);
+    dh.load(reinterpret_cast<const E*>(p.dh) + row * p.ld_dh + i0, p.dh != nullptr ? n : 0, step);
+    rstd = row < p.rows ? __ldg(p.rstd + row) : 0.f;
+  };
+  int turn = 0;
+  const int64_t stride = (int64_t)gridDim.x * side;
+  int64_t group = (int64_t)blockIdx.x * side;
+  load(group + threadIdx.y);
+  for (; group < p.rows; group += stride, turn ^= 1) {
+    const int64_t row = group + threadIdx.y;
+    float g[8], hat[8];
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hat[j] = h.get(j) * rstd;
+      acc[j] = fmaf(dy.get(j), hat[j], acc[j]);
+      g[j] = dy.get(j) * w[j];
+      sum = fmaf(g[j], hat[j], sum);
+    }
+    const Raw<BF16, VEC> d = dh;
+    const float r = rstd;
+    load(row + stride);
+    const float mean = row_reduce<false>(sum, slots.v[turn]) * p.inv_width;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = fmaf(r, g[j] - hat[j] * mean, d.get(j));
+    if (row < p.rows) store8<BF16, VEC>(g, p.dx, row * (int64_t)p.width + i0, left, step);
+  }
+  if (side > 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_acc[(threadIdx.y * 8 + j) * step + threadIdx.x] = acc[j];
+    __syncthreads();
+    if (threadIdx.y != 0) return;
+    for (int y = 1; y < side; ++y)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += s_acc[(y * 8 + j) * step + threadIdx.x];
+  }
+  store8<false, VEC>(acc, p.dw, (int64_t)blockIdx.x * p.width + i0, left, step);
+}
+
+// The same for rows of more than 8192 values: a block's rows are read twice, the second time from L2, and its part of dw
+// lies in shared memory.
+template <bool BF16, bool VEC>
+__global__ void __launch_bounds__(1024) rms_norm_backward_wide_kernel(const NormBwdParams p) {
+  __shared__ __align__(16) Slots slots;
+  extern __shared__ float s_acc[];       // (8 * chunks, threads)
   const int step = blockDim.x, span = 8 * step;
   const int first = (VEC ? 8 : 1) * (int)threadIdx.x;
-  float acc[NC][8];
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[c][j] = 0.f;
+  const int chunks = (p.width + span - 1) / span;
+  for (int k = 0; k < 8 * chunks; ++k) s_acc[k * step + threadIdx.x] = 0.f;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const float rstd = __ldg(p.rstd + row);
-    float g[NC][8], hat[NC][8];
-    float sum = 0.f;
+    float g[8], hat[8], w[8], sum = 0.f;
+    auto load = [&](int c) {
+      const int i0 = first + c * span, left = p.width - i0;
+      load8<BF16, VEC>(g, p.dy, row * p.ld_dy + i0, left, step);
+      load8<BF16, VEC>(hat, p.h, row * p.ld_h + i0, left, step);
+      if (p.w_bf16) load8<true, VEC>(w, p.w, i0, left, step);
+      else load8<false, VEC>(w, p.w, i0, left, step);
+    };
+    for (int c = 0; c < chunks; ++c) {
+      load(c);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int i0 = first + c * span;
-      load8<BF16, VEC>(g[c], p.dy, row * p.ld_dy, i0, step, p.width);
-      load8<BF16, VEC>(hat[c], p.h, row * p.ld_h, i0, step, p.width);
-      float w[8];
-      if (p.w_bf16) load8<true, VEC>(w, p.w, 0, i0, step, p.width);
-      else load8<false, VEC>(w, p.w, 0, i0, step, p.width);
+      for (int j = 0; j < 8; ++j) sum = fmaf(g[j] * w[j], hat[j] * rstd, sum);
+    }
+    const float mean = row_reduce<false>(sum, slots.v[turn]) * p.inv_width;
+    for (int c = 0; c < chunks; ++c) {
+      load(c);
+      const int i0 = first + c * span, left = p.width - i0;
+      float d[8];
+      load8<BF16, VEC>(d, p.dh, row * p.ld_dh + i0, p.dh != nullptr ? left : 0, step);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        hat[c][j] *= rstd;
-        acc[c][j] = fmaf(g[c][j], hat[c][j], acc[c][j]);
-        g[c][j] *= w[j];
-        sum = fmaf(g[c][j], hat[c][j], sum);
+        hat[j] *= rstd;
+        s_acc[(8 * c + j) * step + threadIdx.x] += g[j] * hat[j];
+        d[j] = fmaf(rstd, g[j] * w[j] - hat[j] * mean, d[j]);
       }
-    }
-    // two sets of slots: the next row writes the other one while slower warps still read this one
-    const float mean = row_reduce<false>(sum, slots[turn]) / (float)p.width;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int i0 = first + c * span;
-      float d[8];
-      if (p.dh != nullptr) {
-        load8<BF16, VEC>(d, p.dh, row * p.ld_dh, i0, step, p.width);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = fmaf(rstd, g[c][j] - hat[c][j] * mean, d[j]);
-      store8<BF16, VEC>(d, p.dx, row * (int64_t)p.width, i0, step, p.width);
+      store8<BF16, VEC>(d, p.dx, row * (int64_t)p.width + i0, left, step);
     }
   }
+  for (int c = 0; c < chunks; ++c) {
+    float a[8];
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-    store8<false, VEC>(acc[c], p.dw, (int64_t)blockIdx.x * p.width, first + c * span, step, p.width);
+    for (int j = 0; j < 8; ++j) a[j] = s_acc[(8 * c + j) * step + threadIdx.x];
+    store8<false, VEC>(a, p.dw, (int64_t)blockIdx.x * p.width + first + c * span, p.width - first - c * span, step);
+  }
 }
 
-// out[c] = sum over r of partial[r, c]; 32 columns a block, the rows dealt to 8 warps and joined in a fixed order
+// out[c] = sum over r of partial[r, c]; 32 columns a block, the rows dealt to 16 warps and joined in a fixed order
 __global__ void column_sum_kernel(const float* __restrict__ partial, int rows, int width, float* __restrict__ out) {
-  __shared__ float s[8][32];
+  __shared__ float s[16][32];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float t = 0.f;
-  if (c < width)
-    for (int r = threadIdx.y; r < rows; r += 8) t += partial[(int64_t)r * width + c];
+  if (c < width) {
+#pragma unroll 8
+    for (int r = threadIdx.y; r < rows; r += 16) t += partial[(int64_t)r * width + c];
+  }
   s[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
   if (threadIdx.y == 0 && c < width) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += s[k][threadIdx.x];
+    for (int k = 1; k < 16; ++k) t += s[k][threadIdx.x];
     out[c] = t;
   }
 }
@@ -407,9 +565,9 @@ __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
   const int i0 = (VEC ? 8 : 1) * (int)threadIdx.x + 8 * step * (int)blockIdx.y;
   const int64_t row = blockIdx.x;
   float d[8], g[8], u[8];
-  load8<BF16, VEC>(d, p.dy, row * p.ld_dy, i0, step, p.width);
-  load8<BF16, VEC>(g, p.gate, row * p.ld_gate, i0, step, p.width);
-  load8<BF16, VEC>(u, p.up, row * p.ld_up, i0, step, p.width);
+  load8<BF16, VEC>(d, p.dy, row * p.ld_dy + i0, p.width - i0, step);
+  load8<BF16, VEC>(g, p.gate, row * p.ld_gate + i0, p.width - i0, step);
+  load8<BF16, VEC>(u, p.up, row * p.ld_up + i0, p.width - i0, step);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float sig = __fdividef(1.f, 1.f + __expf(-g[j]));
@@ -418,8 +576,8 @@ __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
     u[j] = ds * g[j];
     g[j] = dg;
   }
-  store8<BF16, VEC>(g, p.dgate, row * p.ld_dgate, i0, step, p.width);
-  store8<BF16, VEC>(u, p.dup, row * p.ld_dup, i0, step, p.width);
+  store8<BF16, VEC>(g, p.dgate, row * p.ld_dgate + i0, p.width - i0, step);
+  store8<BF16, VEC>(u, p.dup, row * p.ld_dup + i0, p.width - i0, step);
 }
 
 // ---------------------------------------------------------------------------
@@ -431,29 +589,50 @@ bool aligned16(const void* ptr, int64_t ld, int elem) {
 
 int round32(int x) { return (x + 31) & ~31; }
 
+int block_shift(int block) { return block == 128 ? 7 : block == 64 ? 6 : 5; }
+
+// Threads and values a thread (8 * NC), by the row's width, and rows a block.  Measured at 32768 x 4096 bf16, block 64,
+// with a residual: 256 threads x 16 values with the next row on its way 149 us (6.30 TB/s), without 172 us; 128 threads x
+// 32 values 215 us; 8 rows a block 149 us, 16 rows 155 us, 1 row 230 us (nothing ahead, and the exponents leave as single
+// bytes).  Narrower rows want more of them: 16384 x 1024 27 us with 8 rows, 24 us with 16.  A row of more than 8192 values
+// takes 32 a thread and no load ahead (registers).  The gated block form has no row statistic: 128 threads x 8 values
+// walk 16 rows of 1024 columns, 16384 x 11008 170 us (5.3 TB/s), 256 threads 175 us; reading and writing bf16 values too
+// 212 us (5.9 TB/s).
 template <int OP, bool BF16, bool VEC, bool BLOCK>
 int launch_row(const RowParams& p, cudaStream_t stream) {
+  constexpr bool kSplit = OP != OP_NORM && BLOCK;       // the row's columns over several blocks
   const int units = (p.width + 7) / 8;
-  int nc, threads, rows_per_block = 1, col_blocks = 1;
-  if (OP != OP_NORM && BLOCK) {
+  int nc, threads, col_blocks = 1;
+  if (kSplit) {
     nc = 1;
-    threads = units < 256 ? round32(units) : 256;
-    col_blocks = (units + threads - 1) / threads;
+    // even shares of up to 128 threads, in multiples of four scale blocks (a word of packed scale factors)
+    const int grain = p.block == 128 ? 64 : 32;
+    col_blocks = (units + 127) / 128;
+    threads = ((units + col_blocks - 1) / col_blocks + grain - 1) / grain * grain;
   } else {
-    nc = units <= 512 ? 1 : units <= 1024 ? 2 : units <= 4096 ? 4 : 0;
-    threads = nc ? round32((units + nc - 1) / nc) : 1024;
+    nc = units <= 64 ? 1 : units <= 1024 ? 2 : units <= 4096 ? 4 : 0;
+    threads = nc == 0 ? 1024 : units <= 16 ? 16 : round32((units + nc - 1) / nc);
   }
-  if (threads <= 128) rows_per_block = 256 / threads;
-  if (rows_per_block > p.rows) rows_per_block = (int)p.rows;
-  const dim3 grid((unsigned)((p.rows + rows_per_block - 1) / rows_per_block), (unsigned)col_blocks);
-  const dim3 block((unsigned)threads, (unsigned)rows_per_block);
-  if (nc == 1) row_quant_kernel<OP, BF16, VEC, BLOCK, 1><<<grid, block, 0, stream>>>(p);
-  if constexpr (OP == OP_NORM || !BLOCK) {
-    if (nc == 2) row_quant_kernel<OP, BF16, VEC, BLOCK, 2><<<grid, block, 0, stream>>>(p);
-    if (nc == 4) row_quant_kernel<OP, BF16, VEC, BLOCK, 4><<<grid, block, 0, stream>>>(p);
+  int side = threads < 256 && !kSplit ? 256 / threads : 1;
+  if (side > p.rows) side = threads == 16 ? (int)((p.rows + 1) & ~1) : (int)p.rows;      // whole warps
+  // first enough blocks for every SM, twice over; then as many rows as are worth it
+  const int64_t resident = (int64_t)sm_count() * 2 * ((nc == 1 ? 1536 : 1024) / (threads * side));
+  const int64_t fair = (p.rows * col_blocks + resident - 1) / resident;
+  const int most = kSplit ? 16 : p.width >= 4096 ? 8 : p.width <= 1024 ? 32 : 32768 / p.width;
+  const int block_rows = (int)(fair < most ? fair : most);
+  const int turns = (block_rows + side - 1) / side;
+  const dim3 grid((unsigned)((p.rows + turns * side - 1) / (turns * side)), (unsigned)col_blocks);
+  const dim3 block((unsigned)threads, (unsigned)side);
+  const size_t smem = BLOCK ? (size_t)nc * threads * 8 / p.block * turns * side : 0;
+#define ROW(NC) row_quant_kernel<OP, BF16, VEC, BLOCK, NC><<<grid, block, smem, stream>>>(p, turns)
+  if (nc == 1) ROW(1);
+  if constexpr (!kSplit) {
+    if (nc == 2) ROW(2);
+    if (nc == 4) ROW(4);
+    if constexpr (OP != OP_NORM)
+      if (nc == 0) ROW(0);
   }
-  if constexpr (OP != OP_NORM && !BLOCK)
-    if (nc == 0) row_quant_kernel<OP, BF16, VEC, BLOCK, 0><<<grid, block, 0, stream>>>(p);
+#undef ROW
   CUDA_TRY(cudaGetLastError());
   return TCFP_OK;
 }
@@ -489,22 +668,43 @@ int dispatch_row(const RowParams& p, cudaStream_t stream) {
   return vec ? launch_row<OP, BF16, true, false>(p, stream) : launch_row<OP, BF16, false, false>(p, stream);
 }
 
-template <bool BF16, bool VEC>
-int launch_norm_bwd(const NormBwdParams& p, int blocks, cudaStream_t stream) {
-  const int units = (p.width + 7) / 8;
-  const int nc = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
-  const int threads = round32((units + nc - 1) / nc);
-  if (nc == 1) rms_norm_backward_kernel<BF16, VEC, 1><<<blocks, threads, 0, stream>>>(p);
-  else if (nc == 2) rms_norm_backward_kernel<BF16, VEC, 2><<<blocks, threads, 0, stream>>>(p);
-  else rms_norm_backward_kernel<BF16, VEC, 4><<<blocks, threads, 0, stream>>>(p);
-  CUDA_TRY(cudaGetLastError());
-  return TCFP_OK;
+constexpr int kNormBwdWidth = 8192;      // 8 values for each of 1024 threads
+
+// threads of a row, rows side by side and blocks of the norm's backward pass: one set of resident blocks
+struct NormBwdShape {
+  int threads, side, blocks;
+};
+NormBwdShape norm_bwd_shape(int64_t rows, int64_t width) {
+  const int units = (int)((width + 7) / 8);
+  NormBwdShape s;
+  s.threads = units > 1024 ? 1024 : units <= 16 ? 16 : round32(units);
+  s.side = s.threads < 256 ? 256 / s.threads : 1;
+  const int64_t groups = (rows + s.side - 1) / s.side;
+  const int64_t resident = (int64_t)sm_count() * (width > kNormBwdWidth ? 1 : 1024 / (s.threads * s.side));
+  s.blocks = (int)(groups < resident ? groups : resident);
+  return s;
 }
 
-
-int norm_bwd_blocks(int64_t rows) {
-  const int64_t most = 4 * (int64_t)sm_count();
-  return (int)(rows < most ? rows : most);
+template <bool BF16, bool VEC>
+int launch_norm_bwd(const NormBwdParams& p, const NormBwdShape& s, cudaStream_t stream) {
+  if (p.width <= kNormBwdWidth) {
+    const size_t smem = s.side > 1 ? (size_t)s.side * s.threads * 8 * sizeof(float) : 0;
+    rms_norm_backward_kernel<BF16, VEC><<<s.blocks, dim3(s.threads, s.side), smem, stream>>>(p);
+  } else {
+    const int smem = (p.width + 8191) / 8192 * 8192 * (int)sizeof(float);
+    static bool done[64] = {false};
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(TCFP_ERR_UNSUPPORTED, "device index %d out of range", dev);
+    if (!done[dev]) {
+      CUDA_TRY(cudaFuncSetAttribute(rms_norm_backward_wide_kernel<BF16, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kMaxNormWidth * (int)sizeof(float)));
+      done[dev] = true;
+    }
+    rms_norm_backward_wide_kernel<BF16, VEC><<<s.blocks, s.threads, smem, stream>>>(p);
+  }
+  CUDA_TRY(cudaGetLastError());
+  return TCFP_OK;
 }
 
 }  // namespace
@@ -522,7 +722,7 @@ extern "C" int32_t tcfp_add_rms_norm_quantize(const void* x, int64_t ld_x, const
   if (w_dtype != TCFP_F32 && w_dtype != TCFP_BF16) return fail(TCFP_ERR_INVALID, "tcfp_add_rms_norm_quantize: weight dtype %d", w_dtype);
   if (residual && !h_out) return fail(TCFP_ERR_INVALID, "tcfp_add_rms_norm_quantize: a residual needs h_out");
   RowParams p{x, residual, ld_x, ld_residual, weight, w_dtype == TCFP_BF16, eps, h_out, rstd_out, codes, ld_codes, scale_out,
-              sf_out, reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, block_size};
+              sf_out, reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, block_size, block_shift(block_size), 1.f / (float)width};
   const int rc = check_row("tcfp_add_rms_norm_quantize", p, dtype, dtype == TCFP_BF16 ? 2 : 4);
   if (rc != TCFP_OK) return rc;
   return dtype == TCFP_BF16 ? dispatch_row<OP_NORM, true>(p, (cudaStream_t)stream) : dispatch_row<OP_NORM, false>(p, (cudaStream_t)stream);
@@ -534,7 +734,7 @@ extern "C" int32_t tcfp_silu_mul_quantize(const void* gate, int64_t ld_gate, con
   if (!up) return fail(TCFP_ERR_INVALID, "tcfp_silu_mul_quantize: NULL argument");
   if (width > kMaxGateWidth) return fail(TCFP_ERR_UNSUPPORTED, "tcfp_silu_mul_quantize: width %lld", (long long)width);
   RowParams p{gate, up, ld_gate, ld_up, nullptr, 0, 0.f, nullptr, nullptr, codes, ld_codes, scale_out, sf_out,
-              reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, block_size};
+              reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, block_size, block_shift(block_size), 1.f / (float)width};
   const int rc = check_row("tcfp_silu_mul_quantize", p, dtype, dtype == TCFP_BF16 ? 2 : 4);
   if (rc != TCFP_OK) return rc;
   return dtype == TCFP_BF16 ? dispatch_row<OP_GATE, true>(p, (cudaStream_t)stream) : dispatch_row<OP_GATE, false>(p, (cudaStream_t)stream);
@@ -544,7 +744,7 @@ extern "C" int32_t tcfp_int8_quantize_rows(const void* x, int64_t ld_x, int32_t 
                                            float* scale_out, void* deq_bf16_out, int64_t rows, int64_t width, void* stream) {
   if (width > kMaxGateWidth) return fail(TCFP_ERR_UNSUPPORTED, "tcfp_int8_quantize_rows: width %lld", (long long)width);
   RowParams p{x, nullptr, ld_x, 0, nullptr, 0, 0.f, nullptr, nullptr, codes, ld_codes, scale_out, nullptr,
-              reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, 0};
+              reinterpret_cast<__nv_bfloat16*>(deq_bf16_out), rows, (int)width, 0, block_shift(0), 1.f / (float)width};
   const int rc = check_row("tcfp_int8_quantize_rows", p, dtype, dtype == TCFP_BF16 ? 2 : 4);
   if (rc != TCFP_OK) return rc;
   return dtype == TCFP_BF16 ? dispatch_row<OP_COPY, true>(p, (cudaStream_t)stream) : dispatch_row<OP_COPY, false>(p, (cudaStream_t)stream);
@@ -552,7 +752,7 @@ extern "C" int32_t tcfp_int8_quantize_rows(const void* x, int64_t ld_x, int32_t 
 
 extern "C" size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
   if (rows < 1 || width < 1 || width > kMaxNormWidth) return 0;
-  return (size_t)norm_bwd_blocks(rows) * (size_t)width * sizeof(float);
+  return (size_t)norm_bwd_shape(rows, width).blocks * (size_t)width * sizeof(float);
 }
 
 extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h, int64_t ld_h, const float* rstd,
@@ -566,16 +766,17 @@ extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const v
   if (rows < 1 || width < 1) return fail(TCFP_ERR_INVALID, "%s: %lld rows, width %lld", what, (long long)rows, (long long)width);
   if (width > kMaxNormWidth) return fail(TCFP_ERR_UNSUPPORTED, "%s: width %lld above %d", what, (long long)width, kMaxNormWidth);
   const int e = dtype == TCFP_BF16 ? 2 : 4;
-  const int blocks = norm_bwd_blocks(rows);
+  const NormBwdShape shape = norm_bwd_shape(rows, width);
+  const int blocks = shape.blocks;
   NormBwdParams p{dy, h, dh, ld_dy, ld_h, ld_dh, rstd, weight, w_dtype == TCFP_BF16, dx,
-                  blocks == 1 ? dw : reinterpret_cast<float*>(workspace), rows, (int)width};
+                  blocks == 1 ? dw : reinterpret_cast<float*>(workspace), rows, (int)width, 1.f / (float)width};
   const bool vec = width % 8 == 0 && aligned16(dy, ld_dy, e) && aligned16(h, ld_h, e) && (!dh || aligned16(dh, ld_dh, e)) &&
                    aligned16(weight, 0, 1) && aligned16(dx, 0, 1) && aligned16(p.dw, 0, 1);
   int rc;
-  if (dtype == TCFP_BF16) rc = vec ? launch_norm_bwd<true, true>(p, blocks, stream) : launch_norm_bwd<true, false>(p, blocks, stream);
-  else rc = vec ? launch_norm_bwd<false, true>(p, blocks, stream) : launch_norm_bwd<false, false>(p, blocks, stream);
+  if (dtype == TCFP_BF16) rc = vec ? launch_norm_bwd<true, true>(p, shape, stream) : launch_norm_bwd<true, false>(p, shape, stream);
+  else rc = vec ? launch_norm_bwd<false, true>(p, shape, stream) : launch_norm_bwd<false, false>(p, shape, stream);
   if (rc != TCFP_OK || blocks == 1) return rc;
-  column_sum_kernel<<<(unsigned)((width + 31) / 32), dim3(32, 8), 0, stream>>>(p.dw, blocks, (int)width, dw);
+  column_sum_kernel<<<(unsigned)((width + 31) / 32), dim3(32, 16), 0, stream>>>(p.dw, blocks, (int)width, dw);
   CUDA_TRY(cudaGetLastError());
   return TCFP_OK;
 }
