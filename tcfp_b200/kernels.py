@@ -14,6 +14,8 @@ and ``out_dtype``.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _C
@@ -501,7 +503,7 @@ class QuantizedActivation:
 
     def __init__(self, codes, scales, block_size, shape, dtype, bf16=None):
         self.codes, self.scales, self.block_size = codes, scales, block_size
-        self.shape, self.dtype, self.bf16 = torch.Size(shape), dtype, bf16
+        self.shape, self.dtype, self.bf16 = shape, dtype, bf16
         # stands for the activation in the autograd graph (see nn.add_rms_norm); its values are never read
         self._handle = None
 
@@ -527,18 +529,20 @@ def _rows_of(t: torch.Tensor, who: str, name: str) -> tuple[torch.Tensor, int]:
     if not t.is_cuda:
         raise RuntimeError(f"{who}: tcfp_b200 runs on CUDA (sm_100) tensors only, got a {t.device} {name}")
     _C.dtype_code(t)
-    if t.ndim == 0 or t.shape[-1] == 0:
-        raise ValueError(f"{who}: {name} needs a last dimension of at least 1, got shape {tuple(t.shape)}")
-    t = t.detach()
-    if t.ndim != 2:
-        rows = 1
-        for n in t.shape[:-1]:
-            rows *= n
-        t = t.reshape(rows, t.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{who}: {name} needs a last dimension of at least 1, got shape {tuple(shape)}")
+    if t.requires_grad:
+        t = t.detach()
+    if len(shape) != 2:
+        t = t.reshape(math.prod(shape[:-1]), shape[-1])
+    rows, width = t.shape
+    ld, unit = t.stride()
+    if unit != 1 and width > 1:
         t = t.contiguous()
+        ld = width
     # the pitch of a single row is never used: give it one that does not stand in the way of wide accesses
-    return t, t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 16) * 16
+    return t, ld if rows > 1 else -(-width // 16) * 16
 
 
 def _same(t: torch.Tensor | None, like: torch.Tensor, who: str, name: str, like_name: str) -> None:
@@ -551,16 +555,20 @@ def _vector(t: torch.Tensor, n: int, device, who: str, name: str, dtypes=(torch.
     if t.shape != (n,) or t.dtype not in dtypes or t.device != device:
         raise ValueError(f"{who}: {name} must be a ({n},) tensor of {' or '.join(str(d) for d in dtypes)} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.detach().contiguous()
+    if t.requires_grad:
+        t = t.detach()
+    return t.contiguous()
 
 
 def _launch(device: torch.device, fn, *args) -> None:
     """Calls a C entry point on ``device``'s current stream."""
-    if device.index == torch.cuda.current_device():
-        _C.check(fn(*args, _C.stream()))
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
-            _C.check(fn(*args, _C.stream()))
+            rc = fn(*args, _C.stream())
+    if rc != 0:
+        _C.check(rc)
 
 
 def _pitch16(t: torch.Tensor, ld: int) -> bool:
@@ -577,20 +585,24 @@ def _check_block(block_size, width: int, who: str) -> None:
 
 
 def _alloc_quantized(x: torch.Tensor, rows: int, width: int, block_size, want_bf16: bool, shape) -> tuple:
-    """The outputs of a row quantizer: ``(QuantizedActivation, sf or None)``."""
-    dev = x.device
-    deq = torch.empty((rows, width), dtype=torch.bfloat16, device=dev) if want_bf16 else None
+    """The outputs of a row quantizer: ``(QuantizedActivation, sf or None,
+    row pitch of the codes)``."""
+    deq = x.new_empty((rows, width), dtype=torch.bfloat16) if want_bf16 else None
     if block_size is not None:
-        codes = torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty((width // block_size, rows), dtype=torch.int8, device=dev)
-        sf = _alloc_sf(rows, width, block_size, dev)
+        codes = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
+        scales = x.new_empty((width // block_size, rows), dtype=torch.int8)
+        sf = _alloc_sf(rows, width, block_size, x.device)
         _attach_sf(scales, sf, block_size)
+        pitch = width
     else:
         # the int8 product reads rows that start on 16-byte boundaries
-        codes = torch.empty((rows, -(-width // 16) * 16), dtype=torch.int8, device=dev)[:, :width]
-        scales = torch.empty(rows, dtype=torch.float32, device=dev)
+        pitch = -(-width // 16) * 16
+        codes = x.new_empty((rows, pitch), dtype=torch.int8)
+        if pitch != width:
+            codes = codes[:, :width]
+        scales = x.new_empty(rows, dtype=torch.float32)
         sf = None
-    return QuantizedActivation(codes, scales, block_size, shape, x.dtype, deq), sf
+    return QuantizedActivation(codes, scales, block_size, shape, x.dtype, deq), sf, pitch
 
 
 def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5, *,
@@ -619,18 +631,14 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch
             r2d, ld_r = r2d.clone(memory_format=torch.contiguous_format), width
         if w.data_ptr() % 16:
             w = w.clone()
-    q, sf = _alloc_quantized(x, rows, width, block_size, want_bf16, x.shape)
-    h = torch.empty((rows, width), dtype=x.dtype, device=x.device) if residual is not None else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    q, sf, pitch = _alloc_quantized(x, rows, width, block_size, want_bf16, x.shape)
+    h = None if residual is None else x.new_empty(x.shape)
+    rstd = x.new_empty(rows, dtype=torch.float32)
     if rows > 0:
-        _launch(x.device, _C.load().tcfp_add_rms_norm_quantize, _C.ptr(x2d), ld_x, _C.ptr(r2d), ld_r, _C.dtype_code(x2d),
-                _C.ptr(w), _C.dtype_code(w), float(eps), _C.ptr(h), _C.ptr(rstd), _C.ptr(q.codes),
-                _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
-    return q, x if h is None else h.reshape(x.shape), rstd
-
-
-def _codes_pitch(codes: torch.Tensor) -> int:
-    return codes.stride(0) if codes.dtype == torch.int8 else codes.shape[1]
+        _launch(x.device, _C.load().tcfp_add_rms_norm_quantize, x2d.data_ptr(), ld_x, _C.ptr(r2d), ld_r, _C.dtype_code(x2d),
+                w.data_ptr(), _C.dtype_code(w), eps, _C.ptr(h), rstd.data_ptr(), q.codes.data_ptr(), pitch,
+                q.scales.data_ptr(), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
+    return q, x if h is None else h, rstd
 
 
 def add_rms_norm_backward(grad: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor,
@@ -670,7 +678,7 @@ def _gate_up(gate: torch.Tensor, up: torch.Tensor | None, who: str):
             raise ValueError(f"{who}: a packed gate_up needs an even last dimension, got shape {tuple(gate.shape)}")
         width = gate.shape[-1] // 2
         both, ld = _rows_of(gate, who, "gate_up")
-        return both[:, :width], ld, both[:, width:], ld, gate.shape[:-1] + (width,)
+        return both[:, :width], ld, both[:, width:], ld, torch.Size(gate.shape[:-1] + (width,))
     _same(up, gate, who, "up", "gate")
     g2d, ld_g = _rows_of(gate, who, "gate")
     u2d, ld_u = _rows_of(up, who, "up")
@@ -695,11 +703,10 @@ def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor | None = None, *, blo
             g2d, ld_g = g2d.clone(memory_format=torch.contiguous_format), width
         if not _pitch16(u2d, ld_u):
             u2d, ld_u = u2d.clone(memory_format=torch.contiguous_format), width
-    q, sf = _alloc_quantized(gate, rows, width, block_size, want_bf16, shape)
+    q, sf, pitch = _alloc_quantized(gate, rows, width, block_size, want_bf16, shape)
     if rows > 0:
-        _launch(gate.device, _C.load().tcfp_silu_mul_quantize, _C.ptr(g2d), ld_g, _C.ptr(u2d), ld_u, _C.dtype_code(g2d),
-                _C.ptr(q.codes), _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(sf), _C.ptr(q.bf16), rows, width,
-                block_size or 0)
+        _launch(gate.device, _C.load().tcfp_silu_mul_quantize, g2d.data_ptr(), ld_g, u2d.data_ptr(), ld_u, _C.dtype_code(g2d),
+                q.codes.data_ptr(), pitch, q.scales.data_ptr(), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
     return q
 
 
@@ -740,10 +747,10 @@ def int8_quantize_rows(x: torch.Tensor, *, want_bf16: bool = False) -> Quantized
     rows, width = x2d.shape
     if width > _MAX_ROW:
         raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
-    q, _ = _alloc_quantized(x, rows, width, None, want_bf16, x.shape)
+    q, _, pitch = _alloc_quantized(x, rows, width, None, want_bf16, x.shape)
     if rows > 0:
-        _launch(x.device, _C.load().tcfp_int8_quantize_rows, _C.ptr(x2d), ld, _C.dtype_code(x2d), _C.ptr(q.codes),
-                _codes_pitch(q.codes), _C.ptr(q.scales), _C.ptr(q.bf16), rows, width)
+        _launch(x.device, _C.load().tcfp_int8_quantize_rows, x2d.data_ptr(), ld, _C.dtype_code(x2d), q.codes.data_ptr(), pitch,
+                q.scales.data_ptr(), _C.ptr(q.bf16), rows, width)
     return q
 
 
@@ -752,13 +759,14 @@ def _int8_operand(t: torch.Tensor, who: str, name: str) -> tuple[torch.Tensor, i
         raise RuntimeError(f"{who}: tcfp_b200 runs on CUDA (sm_100) tensors only, got a {t.device} {name}")
     if t.dtype != torch.int8 or t.ndim != 2:
         raise TypeError(f"{who}: {name} must be a 2-D int8 tensor, got {t.ndim}-D {t.dtype}")
-    pitch = -(-t.shape[1] // 16) * 16
-    if t.data_ptr() % 16 or (t.shape[1] > 1 and t.stride(1) != 1) or \
-            (t.shape[0] > 1 and (t.stride(0) % 16 or t.stride(0) < t.shape[1])):
-        held = torch.empty((t.shape[0], pitch), dtype=torch.int8, device=t.device)[:, :t.shape[1]]
+    rows, width = t.shape
+    ld, unit = t.stride()
+    pitch = -(-width // 16) * 16
+    if t.data_ptr() % 16 or (unit != 1 and width > 1) or (rows > 1 and (ld % 16 or ld < width)):
+        held = t.new_empty((rows, pitch))[:, :width]
         held.copy_(t)
-        t = held
-    return t, t.stride(0) if t.shape[0] > 1 else pitch
+        return held, pitch
+    return t, ld if rows > 1 else pitch
 
 
 def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor, *,
@@ -782,8 +790,8 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     b_scale = _vector(b_scale, N, a.device, who, "b_scale")
     if bias is not None:
         bias = _vector(bias, N, a.device, who, "bias", (torch.float32, torch.bfloat16)).float()
-    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    out = a.new_empty((M, N), dtype=out_dtype)
     if M > 0:
-        _launch(a.device, _C.load().tcfp_int8_gemm, _C.ptr(a), ld_a, _C.ptr(a_scale), _C.ptr(b), ld_b, _C.ptr(b_scale),
-                _C.ptr(bias), _C.ptr(out), code, M, N, K)
+        _launch(a.device, _C.load().tcfp_int8_gemm, a.data_ptr(), ld_a, a_scale.data_ptr(), b.data_ptr(), ld_b,
+                b_scale.data_ptr(), _C.ptr(bias), out.data_ptr(), code, M, N, K)
     return out

@@ -61,7 +61,7 @@ def test_gate_and_row_entry_point_refusals(lib):
     refused(lib, norm(4096, 64, 4096, 64, 4096, 0, 4096, 0, None, 0, 4096, 4096, None, 4, 64, None), -1, "NULL")
     refused(lib, norm(4096, 64, 4096, 64, 4096, 0, 4096, 0, None, 0, 4096, 4096, 4096, 4, 40000, None), -2, "width")
     assert lib.tcfp_rms_norm_backward_workspace_bytes(0, 64) == 0
-    assert lib.tcfp_rms_norm_backward_workspace_bytes(3, 64) >= 3 * 64 * 4
+    assert lib.tcfp_rms_norm_backward_workspace_bytes(3, 64) >= 64 * 4          # at least one row of partial sums
 
 
 def test_product_entry_point_refusals(lib):
