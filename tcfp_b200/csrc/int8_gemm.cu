@@ -6,9 +6,13 @@
 // sum.  Two kernels on tcgen05.mma kind::i8, both fed by TMA through a ring of 128-byte-wide stages of K:
 //
 //   int8_pair_kernel  prompts: a pair of CTAs (cta_group::2) owns a 256 x 256 output tile, as the FP8 pair kernel does.
+//                     Bound by the tensor pipe: 8192 x 12288 x 4096 252 us, 3.27 Pop/s (98 % of twice the measured bf16
+//                     rate).  The channel scales of a tile wait in shared memory: read from global memory by every
+//                     thread, the epilogue took 7 us a tile and set the pace for K below 2048.
 //   int8_few_kernel   few tokens: bound by the weight's bytes, so the weight takes the 128 rows of the MMA and the tokens
-//                     its 16..256 columns, and the CTAs of a cluster split K; the partial sums meet through distributed
-//                     shared memory.  Integer sums do not depend on the split.
+//                     its 16..128 columns, and the CTAs of a cluster split K; the partial sums meet through distributed
+//                     shared memory.  Integer sums do not depend on the split.  22016 x 4096: 19 us for 1 to 32 tokens
+//                     (4.7 TB/s), 12288 x 4096 12 us (4.2 TB/s).
 //
 // Every wait is bounded; see sm100_ptx.cuh.
 #include <cuda.h>
@@ -32,6 +36,8 @@ struct Int8Params {
   int k_stages;
   int group_m;
   int out_bf16;
+  int stages;        // of the ring (few tokens)
+  int wide_out;      // rows of out start on boundaries of four elements
   unsigned int* status;
 };
 
@@ -75,10 +81,11 @@ __device__ __forceinline__ float scaled(int acc, float s_a, float s_b, float bia
 // ---------------------------------------------------------------------------
 // prompts: CTA pairs, 256 x 256 tiles
 // ---------------------------------------------------------------------------
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr int kPairStageBytes = 2 * kTile;
 constexpr int kPieceBytes = 16384;            // 128 rows x 128 bytes of staged output
-constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 2 * kPieceBytes + 256;
+constexpr int kColumnBytes = 2 * 2 * 256 * 4;   // channel scales and bias of two tiles
+constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 2 * kPieceBytes + kColumnBytes + 256;
 
 template <bool OUT_BF16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -88,7 +95,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + kStages * kPairStageBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * kPieceBytes);
+  float* columns = reinterpret_cast<float*>(staging + 2 * kPieceBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + 2 * kPieceBytes + kColumnBytes);
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kStages);
   const uint32_t bar_tfull = smem_u32(bars + 2 * kStages), bar_tempty = smem_u32(bars + 2 * kStages + 2);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
@@ -198,6 +206,13 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       coords(tile, mb, nb);
       const int row0 = mb * 256 + (int)rank * 128;
       const float s_a = row0 + r_local < p.M ? __ldg(p.s_a + row0 + r_local) : 0.f;
+      // this tile's channel scales and bias; the tile before may still be read from the other half
+      float* s_col = columns + buf * 512;
+      for (int c = threadIdx.x - 64; c < 256; c += 128) {
+        const int n = nb * 256 + c;
+        s_col[c] = n < p.N ? __ldg(p.s_b + n) : 0.f;
+        s_col[256 + c] = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
+      }
       if (!epi_all(mbar_wait(bar_tfull + 8 * buf, buf_phase, abort_flag, p.status))) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
@@ -211,12 +226,15 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa(bar_tempty + 8 * buf, 0));
         }
-        const int n0 = nb * 256 + g * 32;
         float o[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int n = n0 + i < p.N ? n0 + i : p.N - 1;
-          o[i] = scaled((int)v[i], s_a, __ldg(p.s_b + n), p.bias ? __ldg(p.bias + n) : 0.f);
+        for (int c = 0; c < 8; ++c) {
+          const float4 sb = reinterpret_cast<const float4*>(s_col + g * 32)[c];
+          const float4 bi = reinterpret_cast<const float4*>(s_col + 256 + g * 32)[c];
+          o[4 * c] = scaled((int)v[4 * c], s_a, sb.x, bi.x);
+          o[4 * c + 1] = scaled((int)v[4 * c + 1], s_a, sb.y, bi.y);
+          o[4 * c + 2] = scaled((int)v[4 * c + 2], s_a, sb.z, bi.z);
+          o[4 * c + 3] = scaled((int)v[4 * c + 3], s_a, sb.w, bi.w);
         }
         // a staging buffer may be rewritten once the store issued two pieces ago has read it
         if (!OUT_BF16 || (g & 1) == 0) {
@@ -289,25 +307,26 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 template <int NT>
 struct Few {
   static constexpr int kStageBytes = kTile + NT * kStageK;
-  // three CTAs an SM while the tokens are few, so that their loads overlap; then two, then one
-  static constexpr int kStages = NT <= 32 ? 4 : NT <= 128 ? 3 : 4;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+  static constexpr int kPartBytes = NT * 128 * 4;           // the partial sums reuse the stages
+  static constexpr int kMinStages = (kPartBytes + kStageBytes - 1) / kStageBytes > 2 ? (kPartBytes + kStageBytes - 1) / kStageBytes : 2;
   static constexpr uint32_t kTmemCols = NT < 32 ? 32 : NT;
-  static_assert(kStages * kStageBytes >= NT * 128 * 4, "the partial sums reuse the stages");
+  static constexpr int smem(int stages) { return 1024 + stages * kStageBytes + 256; }
 };
+constexpr int kMaxFewStages = 12;                            // of the barriers behind the stages
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+// volatile keeps it behind the cluster barrier
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
 
-// gridDim = (splits, weight tiles, token tiles), cluster = (splits, 1, 1)
-template <int NT>
+// gridDim = (S, weight tiles, token tiles), cluster = (S, 1, 1)
+template <int NT, int S>
 __global__ void __launch_bounds__(kThreads)
 int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Int8Params p) {
   using F = Few<NT>;
-  constexpr int kStages = F::kStages;
+  const int kStages = p.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * F::kStageBytes);
@@ -316,9 +335,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = gridDim.x, rank = blockIdx.x;
+  const int rank = blockIdx.x;
   const int n0 = blockIdx.y * 128, t0 = blockIdx.z * NT;
-  const int ks0 = (int)((int64_t)p.k_stages * rank / splits), ks1 = (int)((int64_t)p.k_stages * (rank + 1) / splits);
+  const int ks0 = p.k_stages * rank / S, ks1 = p.k_stages * (rank + 1) / S;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -377,54 +396,84 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     }
     __syncwarp();
   }
-  const int row = ((warp & 3) << 5) | lane;      // of the weight tile; warps 2-5 cover the four lane quarters of TMEM
-  const int n = n0 + row;
+  // The sums go to shared memory as (token, weight row) and meet there: the CTAs of the cluster take the tokens in turn, a
+  // warp a token, a lane four neighbouring channels.
   const int tokens = min(NT, p.M - t0);
-  int* part = reinterpret_cast<int*>(smem);       // (NT, 128) partial sums, once every load and MMA is done
-  float s_b = 0.f, bias = 0.f;
-  auto put = [&](int t, int acc) {
-    const float v = scaled(acc, __ldg(p.s_a + t0 + t), s_b, bias);
-    const int64_t at = (int64_t)(t0 + t) * p.N + n;
-    if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    else reinterpret_cast<float*>(p.out)[at] = v;
-  };
+  int* part = reinterpret_cast<int*>(smem);       // every load and MMA is done by then
   bool live = true;
   if (warp >= 2) {
-    if (n < p.N) {
-      s_b = __ldg(p.s_b + n);
-      if (p.bias) bias = __ldg(p.bias + n);
-    }
-    live = mbar_wait(bar_done, 0, abort_flag, p.status);
-    live = __all_sync(0xFFFFFFFFu, live);
+    live = epi_all(mbar_wait(bar_done, 0, abort_flag, p.status));
     if (live) {
       tc_fence_after();
-#pragma unroll 1
+      const int row = ((warp & 3) << 5) | lane;   // warps 2-5 cover the four lane quarters of TMEM
       for (int c = 0; c < tokens; c += 32) {
         uint32_t v[32];
         tmem_ld32(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (c + i >= tokens) break;
-          if (splits > 1) part[(c + i) * 128 + row] = (int)v[i];
-          else if (n < p.N) put(c + i, (int)v[i]);
-        }
+        for (int i = 0; i < (NT < 32 ? NT : 32); ++i) part[(c + i) * 128 + row] = (int)v[i];
       }
       tc_fence_before();
     }
   }
-  if (splits > 1) {
-    // every CTA of the cluster sums and writes its share of the tokens
-    __syncwarp();
-    cluster_sync_all();
-    if (warp >= 2 && live && n < p.N) {
-      const uint32_t mine = smem_u32(part) + row * 4;
-      for (int t = rank; t < tokens; t += splits) {
-        int acc = 0;
-        for (int r = 0; r < splits; ++r) acc += ld_cluster_s32(mapa(mine + t * 512, r));
-        put(t, acc);
+  __syncwarp();
+  if constexpr (S > 1) cluster_sync_all();
+  else if (warp >= 2) epi_bar_sync();
+  if (warp >= 2 && live) {
+    const int n = n0 + lane * 4;
+    float s_b[4], bias[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s_b[k] = n + k < p.N ? __ldg(p.s_b + n + k) : 0.f;
+      bias[k] = n + k < p.N && p.bias ? __ldg(p.bias + n + k) : 0.f;
+    }
+    constexpr int kBatch = S >= 8 ? 2 : 16 / S > 8 ? 8 : 16 / S;     // tokens whose sums are on their way at once
+    const uint32_t mine = smem_u32(part) + lane * 16;
+    for (int t = rank + S * (warp - 2); t < tokens; t += 4 * S * kBatch) {
+      int4 v[kBatch][S];
+      float s_a[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int at = min(t + 4 * S * b, tokens - 1);
+        s_a[b] = __ldg(p.s_a + t0 + at);
+#pragma unroll
+        for (int r = 0; r < S; ++r) v[b][r] = ld_cluster_v4(S > 1 ? mapa(mine + at * 512, r) : mine + at * 512);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int at = t + 4 * S * b;
+        if (at >= tokens) break;
+        int acc[4] = {v[b][0].x, v[b][0].y, v[b][0].z, v[b][0].w};
+#pragma unroll
+        for (int r = 1; r < S; ++r) {
+          acc[0] += v[b][r].x; acc[1] += v[b][r].y; acc[2] += v[b][r].z; acc[3] += v[b][r].w;
+        }
+        float o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = scaled(acc[k], s_a[b], s_b[k], bias[k]);
+        const int64_t where = (int64_t)(t0 + at) * p.N + n;
+        if (p.wide_out) {          // N is a multiple of 4: four channels or none
+          if (n < p.N) {
+            if (p.out_bf16) {
+              __nv_bfloat162 lo = __floats2bfloat162_rn(o[0], o[1]), hi = __floats2bfloat162_rn(o[2], o[3]);
+              *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + where) =
+                  make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+            } else {
+              *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + where) = make_float4(o[0], o[1], o[2], o[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + k < p.N) {
+              if (p.out_bf16) reinterpret_cast<__nv_bfloat16*>(p.out)[where + k] = __float2bfloat16_rn(o[k]);
+              else reinterpret_cast<float*>(p.out)[where + k] = o[k];
+            }
+        }
       }
     }
+  }
+  if constexpr (S > 1) {
     __syncwarp();
     cluster_sync_all();   // the others may still be reading this CTA's sums
   }
@@ -485,6 +534,9 @@ int allow_smem(Kernel kern, int bytes, bool (&done)[64]) {
   return TCFP_OK;
 }
 
+constexpr int kSmemLimit = 232448;       // of a block
+constexpr int kSmemSm = 233472;          // of an SM; 1 KB of it goes with every block
+
 struct Operands {
   const int8_t *a, *b;
   int64_t lda, ldb;
@@ -522,26 +574,53 @@ int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
   return TCFP_OK;
 }
 
-template <int NT>
-int launch_few(const Operands& o, const Int8Params& p, int splits, cudaStream_t stream) {
+template <int NT, int S>
+int launch_few(const Operands& o, const Int8Params& p, cudaStream_t stream) {
   CUtensorMap tm_w, tm_x;
   int rc;
   if ((rc = make_map(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.b, p.N, p.K, o.ldb, 128)) != TCFP_OK) return rc;
   if ((rc = make_map(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.a, p.M, p.K, o.lda, NT)) != TCFP_OK) return rc;
   static bool done[64] = {false};
-  if ((rc = allow_smem(int8_few_kernel<NT>, Few<NT>::kSmem, done)) != TCFP_OK) return rc;
+  if ((rc = allow_smem(int8_few_kernel<NT, S>, kSmemLimit, done)) != TCFP_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)splits, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + NT - 1) / NT));
+  cfg.gridDim = dim3(S, (unsigned)((p.N + 127) / 128), (unsigned)((p.M + NT - 1) / NT));
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Few<NT>::kSmem;
+  cfg.dynamicSmemBytes = Few<NT>::smem(p.stages);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
+  attr[0].val.clusterDim = {S, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_few_kernel<NT>, tm_w, tm_x, p));
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_few_kernel<NT, S>, tm_w, tm_x, p));
   return TCFP_OK;
+}
+
+// Splits of K: while the weight tiles alone leave SMs without work.  Measured (us, N x K, tokens: 1, 2, 4, 8 splits):
+// 4096 x 4096, 1: 11.7, 8.3, 6.7, 6.8; 32: 12.1, 8.7, 7.5, 9.2.  12288 x 4096, 1: 14.5, 13.2, 12.0, 14.7; 64: 16.7, 15.2, 15.3,
+// 22.2.  22016 x 4096, 1: 19.3, 19.4, 20.3, 24.8.  4096 x 11008, 1: 27.3, 16.8, 12.6, 10.9.  So up to three blocks an SM with
+// 16 tokens, one and a half with more, whose sums take longer to join.
+template <int NT>
+int launch_few(const Operands& o, Int8Params p, cudaStream_t stream) {
+  using F = Few<NT>;
+  const int64_t tiles = (int64_t)((p.N + 127) / 128) * ((p.M + NT - 1) / NT);
+  const int64_t room = (int64_t)sm_count() * (NT == 16 ? 6 : 3) / 2;
+  int splits = 1;
+  while (splits < 8 && 2 * splits * tiles <= room && 4 * splits <= p.k_stages) splits *= 2;
+  // as many stages as the blocks that share an SM leave room for
+  const int64_t blocks = tiles * splits;
+  const int share = blocks <= sm_count() ? 1 : blocks <= 2 * sm_count() || NT == 128 ? 2 : 3;
+  const int bytes = kSmemSm / share - 1024;
+  int stages = ((bytes < kSmemLimit ? bytes : kSmemLimit) - F::smem(0)) / F::kStageBytes;
+  const int need = (p.k_stages + splits - 1) / splits;
+  stages = stages > need ? need : stages;
+  p.stages = stages > kMaxFewStages ? kMaxFewStages : stages < F::kMinStages ? F::kMinStages : stages;
+  switch (splits) {
+    case 8: return launch_few<NT, 8>(o, p, stream);
+    case 4: return launch_few<NT, 4>(o, p, stream);
+    case 2: return launch_few<NT, 2>(o, p, stream);
+    default: return launch_few<NT, 1>(o, p, stream);
+  }
 }
 
 constexpr int64_t kMaxK = 131071;   // 128 * 128 * K stays below 2^31
@@ -571,17 +650,16 @@ extern "C" int32_t tcfp_int8_gemm(const int8_t* a, int64_t ld_a, const float* s_
   p.k_stages = (int)((K + kStageK - 1) / kStageK);
   p.out_bf16 = out_dtype == TCFP_BF16;
   p.status = device_status_ptr();
-  if (M > 512) return p.out_bf16 ? launch_pair<true>(o, p, stream) : launch_pair<false>(o, p, stream);
-  const int nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-  const int64_t ctas = ((N + 127) / 128) * ((M + nt - 1) / nt);
-  const int64_t room = (int64_t)sm_count() * (nt <= 32 ? 3 : nt <= 128 ? 2 : 1);
-  int splits = 1;
-  while (splits < 8 && 2 * splits * ctas <= room && 4 * splits <= p.k_stages) splits *= 2;
-  switch (nt) {
-    case 16: return launch_few<16>(o, p, splits, stream);
-    case 32: return launch_few<32>(o, p, splits, stream);
-    case 64: return launch_few<64>(o, p, splits, stream);
-    case 128: return launch_few<128>(o, p, splits, stream);
-    default: return launch_few<256>(o, p, splits, stream);
-  }
+  p.wide_out = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  // Tokens a tile: all of them up to 64; beyond, 64 while that leaves no SM two tiles, else 128.  The pairs take over where
+  // tiles of 128 would not all be resident (two an SM), or would share SMs while the pairs need one tile each.  Measured (us,
+  // few / pairs): 4096 x 4096, 256 tokens 11.6 / 16.8, 512: 13.6 / 17.2, 640: 17.9 / 16.9; 12288 x 4096, 128: 16.8 / 19.3, 384: 21.1 /
+  // 28.1, 512: 35.8 / 28.5; 22016 x 4096, 128: 23.7 / 31.5, 256: 39.1 / 32.1; 1024 x 1024, 1024: 6.9 / 10.1.
+  const int64_t rows = (N + 127) / 128, tiles = rows * ((M + 127) / 128), pair_tiles = ((N + 255) / 256) * ((M + 255) / 256);
+  if (M > 64 && tiles > sm_count() && (tiles > 2 * sm_count() || 2 * pair_tiles <= sm_count()))
+    return p.out_bf16 ? launch_pair<true>(o, p, stream) : launch_pair<false>(o, p, stream);
+  if (M <= 16) return launch_few<16>(o, p, stream);
+  if (M <= 32) return launch_few<32>(o, p, stream);
+  if (M <= 64 || rows * ((M + 63) / 64) <= sm_count()) return launch_few<64>(o, p, stream);
+  return launch_few<128>(o, p, stream);
 }
