@@ -1,7 +1,8 @@
 """Benchmark of the TCFP-12 hot path: block-scaled dual-FP8 GEMM at 8192^3.
 
     python bench.py [--gpus N] [--steps K] [--warmup W] [--impl ours|reference]
-                    [--workload gemm|mlp|mlp_large|decoder] [--sp] [--no-extras] [--kernel-table]
+                    [--workload gemm|mlp|mlp_large|decoder] [--sp] [--fused-ops] [--no-extras]
+                    [--kernel-table]
 
 One "step" is one forward pass of the hot path over one batch: the fused
 block-scaled dual GEMM  out = X_q . W_hi^T + X_q . W_lo^T  (both products
@@ -270,7 +271,7 @@ TRAIN_DESC = {
 }
 
 
-def _build_train_workload(name: str, dev, world: int, sp: bool):
+def _build_train_workload(name: str, dev, world: int, sp: bool, fused_ops: bool = False):
     import torch
 
     from tcfp_b200.workloads import build_decoder, build_mlp
@@ -290,7 +291,7 @@ def _build_train_workload(name: str, dev, world: int, sp: bool):
         flop = 2.0 * tokens * d * h * 2 * 5
     else:
         d, seed = 4096, 1005
-        model = build_decoder(sequence_parallel=sp).to(dev)
+        model = build_decoder(sequence_parallel=sp, fused_ops=fused_ops).to(dev)
         opt_cls, lr = torch.optim.AdamW, 3e-4
         shape = (8, 4096, d)
         flop = 2.0 * 8 * 4096 * 4 * (4 * d * d + 3 * d * 11008) * 5
@@ -329,7 +330,7 @@ def _kernel_table(step, top: int = 30) -> dict:
 
 
 def _train_step_extra(name: str, dev, world: int, timed, steps: int, sp: bool = False, kernel_table: bool = False,
-                      single_ms: float | None = None) -> dict:
+                      single_ms: float | None = None, fused_ops: bool = False) -> dict:
     """One tensor-parallel training workload: ms per step with the NCCL
     collectives inside the timed region, the same step with the collectives
     switched off, and their difference (communication not hidden by compute)."""
@@ -337,11 +338,13 @@ def _train_step_extra(name: str, dev, world: int, timed, steps: int, sp: bool = 
 
     from tcfp_b200 import tp
 
-    step, flop = _build_train_workload(name, dev, world, sp)
+    step, flop = _build_train_workload(name, dev, world, sp, fused_ops)
     ms = timed(step, steps, 3) / steps
     res = {"config": TRAIN_DESC[name], "parallelism": (f"tp{world}" + (" sequence-parallel" if sp else "")) if world > 1
            else "single GPU", "ms_per_step": ms, "steps": steps,
            "linear_tflops_effective": flop / (ms * 1e-3) / 1e12, "loss": float(step().item())}
+    if fused_ops:
+        res["fused_ops"] = "norms with the residual additions and the gated activation write the layers' FP8 inputs"
     if kernel_table:
         res["kernel_table"] = _kernel_table(step)
     if world > 1:
@@ -360,7 +363,7 @@ def _train_step_extra(name: str, dev, world: int, timed, steps: int, sp: bool = 
             del step
             torch.cuda.empty_cache()
             with tp.single_rank():
-                step, _ = _build_train_workload(name, dev, 1, False)
+                step, _ = _build_train_workload(name, dev, 1, False, fused_ops)
             with tp.collectives_disabled():
                 single_ms = timed(step, steps, 2) / steps
         res["ms_per_step_single_gpu"] = single_ms
@@ -461,7 +464,8 @@ def run_train_workload(args) -> None:
         dist.init_process_group("nccl", device_id=dev)
     timed = _make_timed(dev, world)
     with ClockSampler(local) as clk:
-        res = _train_step_extra(args.workload, dev, world, timed, args.steps, sp=args.sp, kernel_table=args.kernel_table)
+        res = _train_step_extra(args.workload, dev, world, timed, args.steps, sp=args.sp, kernel_table=args.kernel_table,
+                                fused_ops=args.fused_ops)
     _C.check_device_status()
     if rank == 0:
         print(json.dumps({
@@ -731,6 +735,8 @@ def main() -> None:
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--workload", default="gemm", choices=["gemm", "mlp", "mlp_large", "decoder"])
     ap.add_argument("--sp", action="store_true", help="decoder workload: sequence-parallel form")
+    ap.add_argument("--fused-ops", action="store_true",
+                    help="decoder workload: norm and gated-activation operators that write the layers' 8-bit inputs")
     ap.add_argument("--no-extras", action="store_true", help="headline line only")
     ap.add_argument("--kernel-table", action="store_true",
                     help="with --workload: add the per-kernel device time of two steps (torch profiler) to the line")

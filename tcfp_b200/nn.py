@@ -29,6 +29,9 @@ from .core import (
     to_fp8_e5m2_with_colsum,
 )
 from .kernels import (
+    QuantizedActivation,
+    add_rms_norm_backward,
+    add_rms_norm_quantize,
     bf16_weight_grad,
     block_dequantize_bf16,
     block_quantize_fp8,
@@ -38,8 +41,12 @@ from .kernels import (
     fused_dual_gemm_backward_dx,
     fused_dual_gemm_forward,
     fused_dual_quantize_fp8,
+    int8_matmul,
+    int8_quantize_rows,
     pack_block_scales,
     packed_scale_rows,
+    silu_mul_backward,
+    silu_mul_quantize,
 )
 
 
@@ -280,7 +287,7 @@ class _TCFP12BlockScaledFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, input, weight, bias, scale_block_size, hp_grad_weight, error_state, param_name, abd, srr,
-                update_ef, srr_seed, srr_offset, out_dtype=torch.float32, wq_cache=None, hooks=None):
+                update_ef, srr_seed, srr_offset, out_dtype=torch.float32, wq_cache=None, hooks=None, quantized=None):
         w = _master(weight)
         error_buf = None
         if error_state is not None:
@@ -294,10 +301,14 @@ class _TCFP12BlockScaledFunction(torch.autograd.Function):
             lambda: fused_dual_quantize_fp8(w, bs, error_buf, srr, seed=srr_seed, offset=srr_offset,
                                             update_error=update_ef))
         input_shape = input.shape
-        x2d = _flat2d(input)
-        if x2d.dtype not in (torch.float32, torch.bfloat16):
-            x2d = x2d.float()
-        act_fp8, act_scales = block_quantize_fp8(x2d, bs, torch.float8_e4m3fn)
+        if quantized is not None:
+            # the operator in front of the layer wrote the codes; input only stands for them in the graph
+            act_fp8, act_scales = quantized.codes, quantized.scales
+        else:
+            x2d = _flat2d(input)
+            if x2d.dtype not in (torch.float32, torch.bfloat16):
+                x2d = x2d.float()
+            act_fp8, act_scales = block_quantize_fp8(x2d, bs, torch.float8_e4m3fn)
         sp = None if hooks is None else hooks.sp
         if sp is not None:
             # block scales are local to a row: quantize this rank's tokens, gather codes and exponents
@@ -307,7 +318,7 @@ class _TCFP12BlockScaledFunction(torch.autograd.Function):
                 x2d = sp.gather_rows(x2d.contiguous())
         bias_f = None if bias is None else bias.detach().float().contiguous()
         M, K = act_fp8.shape
-        out2d = torch.empty((M, w_hi.shape[0]), device=x2d.device, dtype=out_dtype)
+        out2d = torch.empty((M, w_hi.shape[0]), device=act_fp8.device, dtype=out_dtype)
         act_sf = pack_block_scales(act_scales, bs)
         pending = []
         for r0, r1 in _row_chunks(M, hooks):
@@ -396,7 +407,113 @@ class _TCFP12BlockScaledFunction(torch.autograd.Function):
                 # the saved codes dequantize exactly to bf16; the FP32 gradient goes in as bf16 head + tail
                 grad_weight = bf16_weight_grad(g2d, block_dequantize_bf16(saved_act, act_scales, bs))
         _wait_all([dx_pending])
-        return (grad_input, grad_weight, grad_bias) + (None,) * 12
+        return (grad_input, grad_weight, grad_bias) + (None,) * 13
+
+
+# ---------------------------------------------------------------------------
+# operators that hand a layer its input in 8 bits (no counterpart in the
+# reference, whose layer quantizes the 16-bit output of a norm or activation)
+# ---------------------------------------------------------------------------
+
+def _stand_in(shape, dtype, device) -> torch.Tensor:
+    """A tensor of one element's storage that carries an activation's shape,
+    type and gradient through the autograd graph; nothing reads its values."""
+    return torch.empty(1, dtype=dtype, device=device).expand(shape)
+
+
+class _AddRMSNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, block_size, box):
+        q, h, rstd = add_rms_norm_quantize(x, weight, residual, eps, block_size=block_size)
+        box.append(q)
+        ctx.save_for_backward(h, rstd, weight)
+        ctx.set_materialize_grads(False)
+        stand_in = _stand_in(x.shape, x.dtype, x.device)
+        return stand_in if residual is None else (stand_in, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, grad_h=None):
+        h, rstd, weight = ctx.saved_tensors
+        if grad is None:               # only the stream was used
+            return grad_h, grad_h if ctx.needs_input_grad[1] else None, None, None, None, None
+        dx, dw = add_rms_norm_backward(grad.to(h.dtype), h, rstd, weight, grad_h)
+        return dx, dx if ctx.needs_input_grad[1] else None, dw.to(weight.dtype), None, None, None
+
+
+class _SiluMulFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up, block_size, box):
+        q = silu_mul_quantize(gate, up, block_size=block_size)
+        box.append(q)
+        ctx.save_for_backward(gate, up)
+        return _stand_in(q.shape, gate.dtype, gate.device)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        gate, up = ctx.saved_tensors
+        d = silu_mul_backward(grad.to(gate.dtype), gate, up)
+        return (d, None, None, None) if up is None else (*d, None, None)
+
+
+class _DequantizeFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, stand_in, q):
+        return q.dequantize()
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad, None
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5, *,
+                 block_size: int | None = None) -> tuple[QuantizedActivation, torch.Tensor]:
+    """``h = x + residual`` and the RMS norm of ``h`` in 8 bits, differentiable:
+    returns ``(q, h)`` (``h`` is ``x`` without a residual).  ``q`` goes to a
+    ``TCFPLinear`` of the same ``scale_block_size`` or, with ``block_size``
+    ``None`` (int8, a scale for each token), to an ``Int8Linear``.  The rounding
+    to 8 bits passes gradients through, as it does inside the layers."""
+    box: list[QuantizedActivation] = []
+    out = _AddRMSNormFunction.apply(x, residual, weight, eps, block_size, box)
+    q = box[0]
+    q._handle, h = (out, x) if residual is None else out
+    return q, h
+
+
+def silu_mul(gate: torch.Tensor, up: torch.Tensor | None = None, *, block_size: int | None = None) -> QuantizedActivation:
+    """``silu(gate) * up`` in 8 bits, differentiable; ``up=None``: ``gate`` is
+    the packed ``(..., 2 * width)`` output of a fused gate/up projection, and
+    its gradient comes back packed."""
+    box: list[QuantizedActivation] = []
+    stand_in = _SiluMulFunction.apply(gate, up, block_size, box)
+    box[0]._handle = stand_in
+    return box[0]
+
+
+def dequantized(q: QuantizedActivation) -> torch.Tensor:
+    """The values of ``q`` as a bf16 tensor in the autograd graph."""
+    return q.dequantize() if q._handle is None else _DequantizeFunction.apply(q._handle, q)
+
+
+class QuantizedRMSNorm(nn.Module):
+    """RMS norm with the residual's addition whose output is the 8-bit input
+    of the layer behind it: ``q, h = norm(x, residual)``.  ``scale_block_size``
+    as in that ``TCFPLinear``; ``None`` for an ``Int8Linear``."""
+
+    def __init__(self, d: int, eps: float = 1e-5, *, scale_block_size: int | None = None, device=None, dtype=None):
+        super().__init__()
+        if scale_block_size is not None and (scale_block_size not in (32, 64, 128) or d % scale_block_size != 0):
+            raise ValueError(f"scale_block_size must be 32, 64 or 128 and divide the width ({d}), got {scale_block_size}")
+        self.eps = eps
+        self.scale_block_size = scale_block_size
+        self.weight = nn.Parameter(torch.ones(d, device=device, dtype=dtype))
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        return add_rms_norm(x, self.weight, residual, self.eps, block_size=self.scale_block_size)
+
+    def extra_repr(self) -> str:
+        return f"{self.weight.shape[0]}, eps={self.eps}, scale_block_size={self.scale_block_size}"
 
 
 # ---------------------------------------------------------------------------
@@ -518,8 +635,27 @@ class TCFPLinear(nn.Module):
     def restore_tcfp(self) -> None:
         self._bf16_fallback = False
 
+    def _check_quantized(self, q: QuantizedActivation) -> None:
+        if self.scale_block_size is None or q.block_size != self.scale_block_size:
+            raise ValueError(f"TCFPLinear with scale_block_size={self.scale_block_size} cannot take an activation quantized "
+                             f"with block_size={q.block_size}")
+        if self.hp_grad_weight:
+            raise ValueError("hp_grad_weight needs the input in 16 or 32 bits: it cannot be combined with a quantized activation")
+        if q.shape[-1] != self.in_features:
+            raise ValueError(f"expected {self.in_features} input features, got {q.shape[-1]}")
+
     @torch.compiler.disable
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor | QuantizedActivation) -> torch.Tensor:
+        """``x``: a tensor, or with block scaling the ``QuantizedActivation`` of
+        an operator in front of the layer (``add_rms_norm``, ``silu_mul``)."""
+        quantized = None
+        if isinstance(x, QuantizedActivation):
+            if self._bf16_fallback or self._warmup_remaining > 0 or not self.use_tensor_cores:
+                x = dequantized(x).to(self.weight.dtype)
+            else:
+                self._check_quantized(x)
+                quantized = x
+                x = x._handle if x._handle is not None else _stand_in(x.shape, x.dtype, x.device)
         if self._bf16_fallback:
             return F.linear(x, self.weight, self.bias)
         if self._warmup_remaining > 0:
@@ -545,7 +681,8 @@ class TCFPLinear(nn.Module):
         if self.mode == TCFPMode.TCFP12 and self.scale_block_size is not None:
             return _TCFP12BlockScaledFunction.apply(
                 x, self.weight, self.bias, self.scale_block_size, self.hp_grad_weight, self._error_state,
-                self._param_name, self.abd, srr, update_ef, self.srr_seed, srr_offset, self.out_dtype, self._wq_cache, self._hooks)
+                self._param_name, self.abd, srr, update_ef, self.srr_seed, srr_offset, self.out_dtype, self._wq_cache, self._hooks,
+                quantized)
         return _TCFP12TensorCoreFunction.apply(
             x, self.weight, self.bias, self.hp_grad_weight, self._error_state, self._param_name,
             self.delayed_scaling, self.abd, srr, update_ef, self.srr_seed, srr_offset, self.out_dtype,
@@ -638,4 +775,83 @@ def convert_to_tcfp(model: nn.Module, mode: TCFPMode = TCFPMode.TCFP12, block_si
         if module.bias is not None:
             new.bias = module.bias
         setattr(model, name, new)
+    return model
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integer layer for answering with a trained model
+# ---------------------------------------------------------------------------
+
+class Int8Linear(nn.Module):
+    """``nn.Linear`` with an int8 weight (one FP32 scale for each output
+    channel) and an int8 input (one for each token): the sums are exact
+    integers.  For inference: there is no backward pass, an input that asks for
+    a gradient is refused.
+
+    The input is a tensor, quantized here, or the ``QuantizedActivation`` that
+    ``add_rms_norm`` / ``silu_mul`` return with ``block_size=None``.  No
+    counterpart in the reference."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, *, out_dtype: torch.dtype = torch.float32,
+                 device=None):
+        super().__init__()
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
+        if not 1 <= in_features <= 131071:
+            raise ValueError(f"in_features ({in_features}) must be in [1, 131071]: the integer sums have 32 bits")
+        self.in_features, self.out_features, self.out_dtype = in_features, out_features, out_dtype
+        # rows padded to 16 bytes, as the product reads them
+        self.register_buffer("weight_codes", torch.zeros(out_features, -(-in_features // 16) * 16, dtype=torch.int8, device=device))
+        self.register_buffer("weight_scale", torch.ones(out_features, dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Module, out_dtype: torch.dtype | None = None) -> "Int8Linear":
+        """From an ``nn.Linear`` or ``TCFPLinear`` on the GPU; the output type is
+        the layer's own unless given (``TCFPLinear.out_dtype``, else the
+        weight's)."""
+        w = linear.weight.detach()
+        if out_dtype is None:
+            out_dtype = getattr(linear, "out_dtype", w.dtype)
+        new = cls(w.shape[1], w.shape[0], linear.bias is not None, out_dtype=out_dtype, device=w.device)
+        q = int8_quantize_rows(w)
+        new.weight_codes[:, :w.shape[1]].copy_(q.codes)
+        new.weight_scale.copy_(q.scales)
+        if linear.bias is not None:
+            new.bias.copy_(linear.bias.detach())
+        return new
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor | QuantizedActivation) -> torch.Tensor:
+        source = x._handle if isinstance(x, QuantizedActivation) else x
+        if source is not None and source.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Int8Linear has no backward pass: run it under torch.no_grad() or on an input without gradient")
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"expected {self.in_features} input features, got {x.shape[-1]}")
+        q = x if isinstance(x, QuantizedActivation) else int8_quantize_rows(x)
+        if q.block_size is not None:
+            raise ValueError(f"Int8Linear takes int8 codes with a scale for each token, got E4M3 codes in blocks of {q.block_size}")
+        w = self.weight_codes
+        if w.shape[1] != self.in_features:
+            w = w[:, :self.in_features]
+        out = int8_matmul(q.codes, w, q.scales, self.weight_scale, bias=self.bias, out_dtype=self.out_dtype)
+        return out if len(q.shape) == 2 else out.reshape(*q.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def convert_to_int8(model: nn.Module, skip_patterns: tuple[str, ...] = ("head",)) -> nn.Module:
+    """Swaps the ``nn.Linear`` and ``TCFPLinear`` children of a model on the GPU
+    for ``Int8Linear`` in place, with the traversal and ``skip_patterns`` of
+    :func:`convert_to_tcfp`.  A layer that communicates in its forward pass
+    (row- or sequence-parallel over more than one rank) is refused."""
+    for name, module in list(model.named_children()):
+        convert_to_int8(module, skip_patterns)
+        if any(pat in name for pat in skip_patterns) or not isinstance(module, (nn.Linear, TCFPLinear)):
+            continue
+        hooks = getattr(module, "_hooks", None)
+        if hooks is not None and (hooks.out_hook is not None or hooks.sp is not None or hooks.sp_out is not None):
+            raise ValueError(f"{name}: a layer that reduces or gathers over ranks in its forward pass has no int8 form")
+        setattr(model, name, Int8Linear.from_linear(module))
     return model

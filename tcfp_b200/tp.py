@@ -380,13 +380,15 @@ class ColumnParallelLinear(nn.Module):
 
             self.inner._hooks = LayerHooks(sp=SequenceParallelIO(group), reserve_sms=comm_sms)
 
-    def forward(self, x: torch.Tensor):
+    def forward(self, x, packed: bool = False):
+        """``x``: a tensor, or the ``QuantizedActivation`` the inner layer takes.
+        ``packed=True``: the parts' local outputs as one tensor."""
         if self.sequence_parallel and not self._sp_fused:
             x = _GatherFromSequenceParallel.apply(x, self.group)
         if self.reduce_input_grad and not self._overlap:
             x = _CopyToParallel.apply(x, self.group)
         y = self.inner(x)
-        if self.fused:
+        if self.fused and not packed:
             return torch.split(y, self.local_sizes, dim=-1)
         return y
 

@@ -1,8 +1,8 @@
 """Synthetic training workloads built from the TCFP-12 layers, for step timing
 on 1/2/4/8 GPUs: the two MLP shapes and the 7B-shaped decoder stack named in
 the benchmark configurations.  Random-init weights, random inputs; attention
-and normalisation are plain torch ops -- only the Linear layers are the
-subject here."""
+is a plain torch op, and so are normalisation and the gated activation unless
+``fused_ops`` asks for the operators that write the layers' 8-bit inputs."""
 from __future__ import annotations
 
 import torch
@@ -10,6 +10,7 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .nn import Int8Linear, add_rms_norm, silu_mul
 from .tp import (ColumnParallelLinear, ParallelMLP, RowParallelLinear, copy_to_parallel,
                  gather_from_sequence_parallel, world_and_rank)
 
@@ -29,9 +30,21 @@ class RMSNorm(nn.Module):
         self.eps = eps
         self.token_sharded = token_sharded
 
+    def _weight(self):
+        return copy_to_parallel(self.weight) if self.token_sharded else self.weight
+
     def forward(self, x):
-        w = copy_to_parallel(self.weight) if self.token_sharded else self.weight
-        return F.rms_norm(x, (x.shape[-1],), w.to(x.dtype), self.eps)
+        return F.rms_norm(x, (x.shape[-1],), self._weight().to(x.dtype), self.eps)
+
+    def quantized(self, x, residual, block_size):
+        """``(q, h)`` of :func:`tcfp_b200.nn.add_rms_norm`."""
+        return add_rms_norm(x, self._weight(), residual, self.eps, block_size=block_size)
+
+
+def _input_block(layer) -> int | None:
+    """The format a parallel layer takes its input in: its scale block, or
+    ``None`` for int8 with a scale for each token."""
+    return None if isinstance(layer.inner, Int8Linear) else layer.inner.scale_block_size
 
 
 class DecoderLayer(nn.Module):
@@ -48,12 +61,19 @@ class DecoderLayer(nn.Module):
     world rows -- each column-parallel group all-gathers its input as FP8 codes
     after quantizing this rank's tokens and reduce-scatters its input gradient
     under the weight-gradient GEMM; each row-parallel layer reduce-scatters its
-    output and all-gathers its output gradient."""
+    output and all-gathers its output gradient.
+
+    ``fused_ops=True``: the residual additions and norms, and the gated
+    activation, are one pass each that ends in the 8-bit input of the layer
+    behind it (``nn.add_rms_norm``, ``nn.silu_mul``).  What differs is that the
+    normalised and gated values are rounded once, to 8 bits, instead of to bf16
+    first.  The layers may then be int8 (``nn.convert_to_int8``) as well."""
 
     def __init__(self, d_model: int, n_heads: int, ffn: int, *, granule: int = 64, sequence_parallel: bool = False,
-                 overlap_chunks: int = 1, **layer_kw):
+                 overlap_chunks: int = 1, fused_ops: bool = False, **layer_kw):
         super().__init__()
         world = _world()
+        self.fused_ops = fused_ops
         assert n_heads % world == 0, "heads must divide over the tensor-parallel ranks"
         self.sp = sequence_parallel and world > 1
         self.head_dim = d_model // n_heads
@@ -71,15 +91,28 @@ class DecoderLayer(nn.Module):
                                       sequence_parallel=self.sp, overlap_chunks=overlap_chunks, **layer_kw)
 
     def forward(self, x):                      # x: (B, T, d) bf16; with sequence parallelism (B*T/world, d)
+        if self.fused_ops:
+            h, delta = self.stream(x, None)
+            return h + delta
+        x = x + self._attention(x, self.norm1(x))
+        gate, up = self.gate_up(self.norm2(x))
+        return x + self.down(F.silu(gate) * up)
+
+    def _attention(self, x, normed):
         B, T = self.batch_shape if self.sp else x.shape[:2]
-        q, k, v = self.qkv(self.norm1(x))          # sequence parallel: the layer gathers its (quantized) input
+        q, k, v = self.qkv(normed)                 # sequence parallel: the layer gathers its (quantized) input
         shp = (B, T, self.heads_local, self.head_dim)
         a = F.scaled_dot_product_attention(q.reshape(shp).transpose(1, 2), k.reshape(shp).transpose(1, 2),
                                            v.reshape(shp).transpose(1, 2), is_causal=True)
-        a = a.transpose(1, 2).reshape(q.shape[:-1] + (self.heads_local * self.head_dim,))
-        x = x + self.o(a)
-        gate, up = self.gate_up(self.norm2(x))
-        return x + self.down(F.silu(gate) * up)
+        return self.o(a.transpose(1, 2).reshape(q.shape[:-1] + (self.heads_local * self.head_dim,)))
+
+    def stream(self, x, delta):
+        """With ``fused_ops``: the block on ``x + delta`` (``delta`` nullable);
+        returns the stream and the block's last output, which the next norm
+        adds."""
+        q, h = self.norm1.quantized(x, delta, _input_block(self.qkv))
+        q, h = self.norm2.quantized(h, self._attention(h, q), _input_block(self.gate_up))
+        return h, self.down(silu_mul(self.gate_up(q, packed=True), block_size=_input_block(self.down)))
 
 
 class Decoder(nn.Module):
@@ -93,9 +126,7 @@ class Decoder(nn.Module):
 
     def forward(self, x):
         if not self.sp:
-            for layer in self.layers:
-                x = layer(x)
-            return x
+            return self._blocks(x)
         B, T, d = x.shape
         world, rank = dist.get_world_size(), dist.get_rank()
         tokens = x.reshape(B * T, d)
@@ -103,15 +134,24 @@ class Decoder(nn.Module):
         h = tokens[rank * rows:(rank + 1) * rows]
         for layer in self.layers:
             layer.batch_shape = (B, T)
-            h = layer(h)
-        return gather_from_sequence_parallel(h).reshape(B, T, d)
+        return gather_from_sequence_parallel(self._blocks(h)).reshape(B, T, d)
+
+    def _blocks(self, x):
+        if not (self.layers and self.layers[0].fused_ops):
+            for layer in self.layers:
+                x = layer(x)
+            return x
+        delta = None
+        for layer in self.layers:
+            x, delta = layer.stream(x, delta)
+        return x + delta
 
 
 def build_decoder(n_layers=4, d_model=4096, n_heads=32, ffn=11008, block=64, *, sequence_parallel=False,
-                  overlap_chunks=1, **layer_kw) -> nn.Module:
+                  overlap_chunks=1, fused_ops=False, **layer_kw) -> nn.Module:
     kw = dict(scale_block_size=block, out_dtype=torch.bfloat16, **layer_kw)
     m = Decoder([DecoderLayer(d_model, n_heads, ffn, granule=block, sequence_parallel=sequence_parallel,
-                              overlap_chunks=overlap_chunks, **kw) for _ in range(n_layers)])
+                              overlap_chunks=overlap_chunks, fused_ops=fused_ops, **kw) for _ in range(n_layers)])
     _name_layers(m)
     _init_weights(m)
     return m
