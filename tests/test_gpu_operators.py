@@ -88,6 +88,8 @@ def check_codes(q, y, rel):
 # ---------------------------------------------------------------------------
 
 ROW_SHAPES = [(1, 4096), (3, 1), (5, 7), (2, 333), (33, 1000), (17, 2731), (130, 64), (9, 5120), (3, 11008), (2, 32768), (1, 32761)]
+# many rows, not a multiple of what a block takes: 2 and 4 chunks a thread, one warp a row and more
+ROW_SHAPES += [(2371, 264), (2371, 512), (2371, 520), (2370, 1024), (2371, 1032), (2371, 2048), (2371, 4096), (2371, 8192)]
 BLOCK_SHAPES = [(1, 128), (33, 384), (130, 4096), (257, 640), (3, 11008), (2, 32768)]
 
 
