@@ -661,28 +661,41 @@ def add_rms_norm_backward(grad: torch.Tensor, h: torch.Tensor, rstd: torch.Tenso
         return torch.empty_like(h), torch.zeros(width, dtype=torch.float32, device=h.device)
     g2d, ld_g = _rows_of(grad, who, "grad")
     d2d, ld_d = (None, 0) if grad_h is None else _rows_of(grad_h, who, "grad_h")
-    dx = torch.empty((rows, width), dtype=h.dtype, device=h.device)
-    dw = torch.empty(width, dtype=torch.float32, device=h.device)
+    dx = h.new_empty(h.shape)
+    dw = h.new_empty(width, dtype=torch.float32)
     lib = _C.load()
-    with torch.cuda.device(h.device):     # the workspace goes by the device's number of SMs
-        ws = torch.empty(lib.tcfp_rms_norm_backward_workspace_bytes(rows, width), dtype=torch.uint8, device=h.device)
-    _launch(h.device, lib.tcfp_rms_norm_backward, _C.ptr(g2d), ld_g, _C.ptr(h2d), ld_h, _C.ptr(rstd), _C.dtype_code(h2d),
-            _C.ptr(w), _C.dtype_code(w), _C.ptr(d2d), ld_d, _C.ptr(dx), _C.ptr(dw), _C.ptr(ws), rows, width)
-    return dx.reshape(h.shape), dw
+    if h.device.index == torch._C._cuda_getDevice():      # the workspace goes by the device's number of SMs
+        nbytes = lib.tcfp_rms_norm_backward_workspace_bytes(rows, width)
+    else:
+        with torch.cuda.device(h.device):
+            nbytes = lib.tcfp_rms_norm_backward_workspace_bytes(rows, width)
+    ws = h.new_empty(nbytes, dtype=torch.uint8)
+    _launch(h.device, lib.tcfp_rms_norm_backward, g2d.data_ptr(), ld_g, h2d.data_ptr(), ld_h, rstd.data_ptr(), _C.dtype_code(h2d),
+            w.data_ptr(), _C.dtype_code(w), _C.ptr(d2d), ld_d, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), rows, width)
+    return dx, dw
 
 
 def _gate_up(gate: torch.Tensor, up: torch.Tensor | None, who: str):
-    """Row views of gate and up: two tensors, or the halves of one packed ``(..., 2 * width)`` tensor."""
+    """Gate and up as ``(rows, width, shape, gate address, pitch, up address,
+    pitch, tensors that hold them)``: two tensors, or the halves of one packed
+    ``(..., 2 * width)`` tensor."""
     if up is None:
-        if gate.ndim == 0 or gate.shape[-1] % 2 != 0:
-            raise ValueError(f"{who}: a packed gate_up needs an even last dimension, got shape {tuple(gate.shape)}")
-        width = gate.shape[-1] // 2
+        shape = gate.shape
+        if not shape or shape[-1] % 2 != 0:
+            raise ValueError(f"{who}: a packed gate_up needs an even last dimension, got shape {tuple(shape)}")
         both, ld = _rows_of(gate, who, "gate_up")
-        return both[:, :width], ld, both[:, width:], ld, torch.Size(gate.shape[:-1] + (width,))
-    _same(up, gate, who, "up", "gate")
-    g2d, ld_g = _rows_of(gate, who, "gate")
-    u2d, ld_u = _rows_of(up, who, "up")
-    return g2d, ld_g, u2d, ld_u, gate.shape
+        rows, width = both.shape[0], shape[-1] // 2
+        at = both.data_ptr()
+        shape = shape[:-1] + (width,)
+        out = rows, width, shape, at, ld, at + width * both.element_size(), ld, both
+    else:
+        _same(up, gate, who, "up", "gate")
+        g2d, ld_g = _rows_of(gate, who, "gate")
+        u2d, ld_u = _rows_of(up, who, "up")
+        out = *g2d.shape, gate.shape, g2d.data_ptr(), ld_g, u2d.data_ptr(), ld_u, (g2d, u2d)
+    if out[1] > _MAX_ROW:
+        raise ValueError(f"{who}: width ({out[1]}) must be at most {_MAX_ROW}")
+    return out
 
 
 _MAX_ROW = 1 << 26
@@ -693,20 +706,18 @@ def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor | None = None, *, blo
     """``silu(gate) * up`` in FP32, quantized, one pass.  ``up=None``: ``gate``
     is the packed ``(..., 2 * width)`` output of a fused gate/up projection."""
     who = "silu_mul_quantize"
-    g2d, ld_g, u2d, ld_u, shape = _gate_up(gate, up, who)
-    rows, width = g2d.shape
+    rows, width, shape, at_g, ld_g, at_u, ld_u, held = _gate_up(gate, up, who)
     _check_block(block_size, width, who)
-    if width > _MAX_ROW:
-        raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
     if block_size is not None:
-        if not _pitch16(g2d, ld_g):
-            g2d, ld_g = g2d.clone(memory_format=torch.contiguous_format), width
-        if not _pitch16(u2d, ld_u):
-            u2d, ld_u = u2d.clone(memory_format=torch.contiguous_format), width
+        e = gate.element_size()
+        if at_g % 16 or at_u % 16 or ld_g * e % 16 or ld_u * e % 16:
+            g2d, u2d = held if up is not None else (held[:, :width], held[:, width:])
+            held = g2d.clone(memory_format=torch.contiguous_format), u2d.clone(memory_format=torch.contiguous_format)
+            at_g, at_u, ld_g, ld_u = held[0].data_ptr(), held[1].data_ptr(), width, width
     q, sf, pitch = _alloc_quantized(gate, rows, width, block_size, want_bf16, shape)
     if rows > 0:
-        _launch(gate.device, _C.load().tcfp_silu_mul_quantize, g2d.data_ptr(), ld_g, u2d.data_ptr(), ld_u, _C.dtype_code(g2d),
-                q.codes.data_ptr(), pitch, q.scales.data_ptr(), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
+        _launch(gate.device, _C.load().tcfp_silu_mul_quantize, at_g, ld_g, at_u, ld_u, _C.dtype_code(gate), q.codes.data_ptr(),
+                pitch, q.scales.data_ptr(), _C.ptr(sf), _C.ptr(q.bf16), rows, width, block_size or 0)
     return q
 
 
@@ -715,26 +726,19 @@ def silu_mul_backward(grad: torch.Tensor, gate: torch.Tensor, up: torch.Tensor |
     the identity: ``(dgate, dup)``, or one packed tensor where ``gate`` is
     packed."""
     who = "silu_mul_backward"
-    g2d, ld_g, u2d, ld_u, shape = _gate_up(gate, up, who)
+    rows, width, shape, at_g, ld_g, at_u, ld_u, held = _gate_up(gate, up, who)
     if grad.shape != shape or grad.dtype != gate.dtype or grad.device != gate.device:
         raise ValueError(f"{who}: grad must be {tuple(shape)} {gate.dtype} on {gate.device}, got {tuple(grad.shape)} "
                          f"{grad.dtype} on {grad.device}")
-    rows, width = g2d.shape
-    if width > _MAX_ROW:
-        raise ValueError(f"{who}: width ({width}) must be at most {_MAX_ROW}")
     d2d, ld_d = _rows_of(grad, who, "grad")
-    if up is None:
-        both = torch.empty((rows, 2 * width), dtype=gate.dtype, device=gate.device)
-        dg, du, ld = both[:, :width], both[:, width:], 2 * width
-    else:
-        dg = torch.empty((rows, width), dtype=gate.dtype, device=gate.device)
-        du, ld = torch.empty_like(dg), width
+    dg = gate.new_empty(gate.shape)
+    du = None if up is None else gate.new_empty(gate.shape)
     if rows > 0:
-        _launch(gate.device, _C.load().tcfp_silu_mul_backward, _C.ptr(d2d), ld_d, _C.ptr(g2d), ld_g, _C.ptr(u2d), ld_u,
-                _C.dtype_code(g2d), _C.ptr(dg), ld, _C.ptr(du), ld, rows, width)
-    if up is None:
-        return both.reshape(gate.shape)
-    return dg.reshape(shape), du.reshape(shape)
+        at = dg.data_ptr()
+        ld = 2 * width if up is None else width
+        _launch(gate.device, _C.load().tcfp_silu_mul_backward, d2d.data_ptr(), ld_d, at_g, ld_g, at_u, ld_u, _C.dtype_code(gate),
+                at, ld, at + width * gate.element_size() if up is None else du.data_ptr(), ld, rows, width)
+    return dg if up is None else (dg, du)
 
 
 def int8_quantize_rows(x: torch.Tensor, *, want_bf16: bool = False) -> QuantizedActivation:

@@ -467,6 +467,7 @@ class _DequantizeFunction(torch.autograd.Function):
         return grad, None
 
 
+@torch.compiler.disable
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5, *,
                  block_size: int | None = None) -> tuple[QuantizedActivation, torch.Tensor]:
     """``h = x + residual`` and the RMS norm of ``h`` in 8 bits, differentiable:
@@ -481,6 +482,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     return q, h
 
 
+@torch.compiler.disable
 def silu_mul(gate: torch.Tensor, up: torch.Tensor | None = None, *, block_size: int | None = None) -> QuantizedActivation:
     """``silu(gate) * up`` in 8 bits, differentiable; ``up=None``: ``gate`` is
     the packed ``(..., 2 * width)`` output of a fused gate/up projection, and
@@ -491,6 +493,7 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor | None = None, *, block_size: 
     return box[0]
 
 
+@torch.compiler.disable
 def dequantized(q: QuantizedActivation) -> torch.Tensor:
     """The values of ``q`` as a bf16 tensor in the autograd graph."""
     return q.dequantize() if q._handle is None else _DequantizeFunction.apply(q._handle, q)
@@ -805,6 +808,16 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_scale", torch.ones(out_features, dtype=torch.float32, device=device))
         self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32, device=device) if bias else None)
 
+    def _apply(self, fn, *args, **kw):
+        # scale and bias stay FP32 when a model is cast to another type
+        held = self.weight_scale, self.bias
+        super()._apply(fn, *args, **kw)
+        for name, old in zip(("weight_scale", "bias"), held):
+            now = getattr(self, name)
+            if now is not None and now.dtype != torch.float32:
+                setattr(self, name, old.to(now.device))
+        return self
+
     @classmethod
     def from_linear(cls, linear: nn.Module, out_dtype: torch.dtype | None = None) -> "Int8Linear":
         """From an ``nn.Linear`` or ``TCFPLinear`` on the GPU; the output type is
@@ -845,10 +858,14 @@ def convert_to_int8(model: nn.Module, skip_patterns: tuple[str, ...] = ("head",)
     """Swaps the ``nn.Linear`` and ``TCFPLinear`` children of a model on the GPU
     for ``Int8Linear`` in place, with the traversal and ``skip_patterns`` of
     :func:`convert_to_tcfp`.  A layer that communicates in its forward pass
-    (row- or sequence-parallel over more than one rank) is refused."""
+    (row- or sequence-parallel over more than one rank) is refused; the output
+    projection of ``nn.MultiheadAttention``, whose weight that module reads
+    itself, stays as it is."""
     for name, module in list(model.named_children()):
         convert_to_int8(module, skip_patterns)
         if any(pat in name for pat in skip_patterns) or not isinstance(module, (nn.Linear, TCFPLinear)):
+            continue
+        if isinstance(module, nn.modules.linear.NonDynamicallyQuantizableLinear):
             continue
         hooks = getattr(module, "_hooks", None)
         if hooks is not None and (hooks.out_hook is not None or hooks.sp is not None or hooks.sp_out is not None):

@@ -318,6 +318,60 @@ def test_convert_to_int8():
     assert isinstance(seq[0], Int8Linear) and isinstance(seq[1][0], Int8Linear) and isinstance(seq.head, torch.nn.Linear)
 
 
+def test_int8_models_survive_casts_and_attention_modules():
+    from tcfp_b200.nn import Int8Linear, convert_to_int8
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.attn = torch.nn.MultiheadAttention(64, 2, batch_first=True)
+            self.fc = torch.nn.Linear(64, 48)
+
+        def forward(self, x):
+            return self.fc(self.attn(x, x, x)[0])
+
+    net = convert_to_int8(Net().to(DEV))
+    assert isinstance(net.fc, Int8Linear) and not isinstance(net.attn.out_proj, Int8Linear)
+    x = rand(26, 2, 5, 64)
+    with torch.no_grad():
+        y = net(x)
+        scale = net.fc.weight_scale.clone()
+        net.to(torch.bfloat16)
+        assert net.fc.weight_scale.dtype == net.fc.bias.dtype == torch.float32 and torch.equal(net.fc.weight_scale, scale)
+        # attention in bf16: 8 bits in and out, a softmax of 5 terms
+        assert rel_fro(net(x.to(torch.bfloat16)), y) <= 0.05
+
+
+def test_sequence_parallel_io_passes_quantized_codes():
+    """With the collectives of one rank the layer's gathers see the codes and planes of the operator."""
+    from tcfp_b200.nn import LayerHooks, add_rms_norm
+    from tcfp_b200.tp import SequenceParallelIO
+
+    class Doubling(SequenceParallelIO):      # two ranks that hold the same tokens
+        def gather_rows(self, t):
+            return torch.cat([t.view(torch.uint8), t.view(torch.uint8)]).view(t.dtype)
+
+        def gather_planes(self, planes):
+            return torch.cat([planes, planes], dim=1)
+
+        def scatter_rows_async(self, full):
+            n = full.shape[0] // 2
+            return None, full[:n] + full[n:]
+
+    lin = layer(128, 64, error_feedback=False)      # with it the second forward quantizes the weight plus the first one's error
+    x = rand(27, 160, 128, dtype=torch.bfloat16).requires_grad_()
+    w = torch.ones(128, device=DEV)
+    y = lin(add_rms_norm(torch.cat([x, x]), w, block_size=64)[0])       # the same number of rows: the same tiles and sums
+    gy = rand(28, 160, 64, dtype=torch.bfloat16)
+    (gx,) = torch.autograd.grad(lin(add_rms_norm(x, w, block_size=64)[0]), x, gy)
+    lin._hooks = LayerHooks(sp=Doubling())
+    z = lin(add_rms_norm(x, w, block_size=64)[0])
+    assert torch.equal(z, y)
+    (gz,) = torch.autograd.grad(z, x, torch.cat([gy, gy]))
+    # twice every gradient, formed by an addition of two equal bf16 numbers: exact until the norm's own rounding
+    assert (gz.float() - 2 * gx.float()).abs().max() <= 2 * 2.0**-8 * gx.float().abs().max()
+
+
 def test_convert_to_int8_refuses_communicating_layers():
     from tcfp_b200.nn import LayerHooks, TCFPLinear, convert_to_int8
 

@@ -444,3 +444,64 @@ def test_another_stream_and_a_captured_graph():
             torch.cuda.synchronize()
             for _, out in graphs:
                 assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams share nothing."""
+    from tcfp_b200 import kernels as K
+
+    w = torch.ones(2048, device=DEV)
+    xs = [stream(50 + i, 1500, 2048, torch.bfloat16) for i in range(2)]
+    b = K.int8_quantize_rows(stream(52, 640, 2048, torch.float32))
+
+    def work(x):
+        q, h, rstd = K.add_rms_norm_quantize(x, w, x)
+        y = K.int8_matmul(q.codes, b.codes, q.scales, b.scales)
+        few = K.int8_matmul(q.codes[:9], b.codes, q.scales[:9], b.scales)
+        return (y, few, *K.add_rms_norm_backward(x, h, rstd, w))
+
+    want = [work(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(5):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(work(x))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+def test_offsets_past_32_bits():
+    """The last rows of tensors of more than 2^31 elements are those of the same rows alone."""
+    from tcfp_b200 import kernels as K
+
+    rows, width = 140_000, 16_384
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=DEV)
+    tail = stream(60, 9, width, torch.bfloat16)
+    x[-9:] = tail
+    w = torch.ones(width, device=DEV)
+    for bs in (None, 64):
+        q, _, rstd = K.add_rms_norm_quantize(x, w, block_size=bs)
+        q9, _, rstd9 = K.add_rms_norm_quantize(tail, w, block_size=bs)
+        assert torch.equal(q.codes[-9:].view(torch.uint8), q9.codes.view(torch.uint8)) and torch.equal(rstd[-9:], rstd9)
+        assert torch.equal(q.scales[-9:] if bs is None else q.scales[:, -9:], q9.scales)
+        assert (q.codes[0].view(torch.uint8) == 0).all()
+        del q
+        g, g9 = K.silu_mul_quantize(x, block_size=bs), K.silu_mul_quantize(tail, block_size=bs)
+        assert torch.equal(g.codes[-9:].view(torch.uint8), g9.codes.view(torch.uint8))
+        del g
+    dx, dw = K.add_rms_norm_backward(x, x, rstd, w)
+    dx9, dw9 = K.add_rms_norm_backward(tail, tail, rstd9, w)
+    assert torch.equal(dx[-9:], dx9) and (dw - dw9).abs().max() <= 1e-5 * dw9.abs().max()      # other rows add zeros in another order
+    del dx
+    d = K.silu_mul_backward(x[:, :width // 2], x)
+    assert torch.equal(d[-9:], K.silu_mul_backward(tail[:, :width // 2], tail))
+    del d, x
+    m, n = 70_000, 32_768
+    a, b = codes(61, m, 64), codes(62, n, 64)
+    sa, sb = torch.rand(m, generator=gen(63)).to(DEV), torch.rand(n, generator=gen(64)).to(DEV)
+    out = K.int8_matmul(a, b, sa, sb, out_dtype=torch.bfloat16)
+    assert torch.equal(out[-300:], K.int8_matmul(a[-300:], b, sa[-300:], sb, out_dtype=torch.bfloat16))
