@@ -353,10 +353,10 @@ int32_t tcfp_bf16_dw_gemm(const void* x, const void* g_hi, const void* g_lo,
  *       (width/bs, rows) and sf_out (nullable) = packed E8M0 copy, by the rule
  *       of tcfp_quantize; rows of all tensors 16-byte aligned.  A NaN stays
  *       NaN, an infinity saturates.
- *   block_size 0: int8 codes = round_half_even(y / s) with one float
- *       s = max(max |y|, 1e-12) / 127 for each row, rounded to FP32, in
- *       scale_out; any alignment and width.  A row that holds a NaN or an
- *       infinity has a scale that is not finite.
+ *   block_size 0: int8 codes = round_half_even(y * (1 / s)) with one float
+ *       s = max(max |y|, 1e-12) / 127 for each row in scale_out; s, its
+ *       reciprocal and the product are rounded to FP32; any alignment and
+ *       width.  A row that holds a NaN or an infinity has the scale NaN.
  * ld_* are row pitches in elements.  ld_codes >= width; what lies between them
  * is not written.  deq_bf16_out (nullable, dense) receives the values the
  * codes stand for, rounded to bf16.  1 <= rows < 2^31, width <= 2^26.

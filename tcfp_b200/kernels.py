@@ -743,8 +743,8 @@ def silu_mul_backward(grad: torch.Tensor, gate: torch.Tensor, up: torch.Tensor |
 
 def int8_quantize_rows(x: torch.Tensor, *, want_bf16: bool = False) -> QuantizedActivation:
     """``(..., width)`` FP32 or bf16 -> int8 codes with one FP32 scale for each
-    row, ``s = max(amax, 1e-12) / 127``, ``code = round(x / s)`` (ties to
-    even): a token's scale for an activation, an output channel's for a weight
+    row, ``s = max(amax, 1e-12) / 127``, ``code = round(x * (1 / s))`` (FP32,
+    ties to even): a token's scale for an activation, an output channel's for a weight
     ``(N, K)``."""
     who = "int8_quantize_rows"
     x2d, ld = _rows_of(x, who, "x")

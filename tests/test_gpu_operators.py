@@ -48,8 +48,8 @@ def check_row_codes(q, y, rel):
     code = q.codes.double()
     assert code.abs().max() <= 127
     off = (code * s[:, None] - y).abs()
-    # half a step, the quotient's rounding, and y's own error
-    assert (off <= s[:, None] * (0.5 + 127 * 2 * U) + rel * y.abs()).all()
+    # half a step, the roundings of the reciprocal and of the product, and y's own error
+    assert (off <= s[:, None] * (0.5 + 127 * 2.001 * U) + rel * y.abs()).all()
     if q.bf16 is not None:
         v = code * s[:, None]
         assert ((q.bf16.double() - v).abs() <= (2.0**-8 + 2 * U) * v.abs()).all()
@@ -89,8 +89,8 @@ def check_codes(q, y, rel):
 
 ROW_SHAPES = [(1, 4096), (3, 1), (5, 7), (2, 333), (33, 1000), (17, 2731), (130, 64), (9, 5120), (3, 11008), (2, 32768), (1, 32761)]
 # many rows, not a multiple of what a block takes: 2 and 4 chunks a thread, one warp a row and more
-ROW_SHAPES += [(2371, 264), (2371, 512), (2371, 520), (2370, 1024), (2371, 1032), (2371, 2048), (2371, 4096), (2371, 8192)]
-BLOCK_SHAPES = [(1, 128), (33, 384), (130, 4096), (257, 640), (3, 11008), (2, 32768)]
+ROW_SHAPES += [(2371, 264), (2371, 512), (2371, 520), (2370, 1024), (2371, 1032), (2371, 2048), (2371, 4096), (2371, 8192), (1201, 8200), (1203, 12296)]
+BLOCK_SHAPES = [(1, 128), (33, 384), (130, 4096), (257, 640), (3, 11008), (2, 32768), (1201, 8320), (907, 32768)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -266,7 +266,7 @@ def test_norm_limits():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("shape", ROW_SHAPES + [(2, 40000), (1, 50001), (5000, 128)])
 def test_int8_quantize_rows(shape, dtype):
-    """The codes are defined to the bit: the quotient in FP32, rounded half to even."""
+    """The codes are defined to the bit: the product with the reciprocal in FP32, rounded half to even."""
     from tcfp_b200.kernels import int8_quantize_rows
 
     x = stream(12, *shape, dtype)
@@ -280,7 +280,8 @@ def test_int8_quantize_rows(shape, dtype):
     f = x.double()
     s = (f.abs().amax(1).float().clamp(min=1e-12).double() / 127).float()
     assert torch.equal(q.scales, s)
-    assert torch.equal(q.codes.float(), torch.round((f / s.double()[:, None]).float()))
+    # the product of two FP32 numbers is exact in 64 bits
+    assert torch.equal(q.codes.float(), torch.round((f * (1 / s.double()).float().double()[:, None]).float()))
     check_row_codes(q, x.double(), 0.0)
     assert q.codes.stride(0) % 16 == 0
 
