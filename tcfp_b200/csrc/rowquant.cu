@@ -285,8 +285,8 @@ __device__ __forceinline__ void flush_exponents(const int8_t* s_e, const RowPara
 // cp.async measured slower: gate 16384 x 11008 to int8 210 -> 233 us, norm to block codes 308 -> 359 us).  The block walks `turns` rows for each of its
 // blockDim.y places.  gridDim.y > 1 (only where no statistic spans the row) splits the row's columns.  NC = 0 walks a
 // row of any width and loads it again for each pass.
-template <int OP, bool BF16, bool VEC, bool BLOCK, int NC>
-__global__ void __launch_bounds__(NC == 1 ? 256 : NC == 2 ? 512 : 1024, NC == 1 ? 6 : NC == 2 ? 2 : 1)
+template <int OP, bool BF16, bool VEC, bool BLOCK, int NC, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : THREADS == 384 ? 3 : THREADS == 512 ? 2 : 1)
 row_quant_kernel(const RowParams p, const int turns) {
   __shared__ __align__(16) Slots s_sum, s_max;
   extern __shared__ int8_t s_e[];
@@ -694,7 +694,7 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
   int side = threads < 256 && !kSplit ? 256 / threads : 1;
   if (side > p.rows) side = threads == 16 ? (int)((p.rows + 1) & ~1) : (int)p.rows;      // whole warps
   // first enough blocks for every SM, twice over; then as many rows as are worth it
-  const int64_t resident = (int64_t)sm_count() * 2 * ((nc == 1 ? 1536 : 1024) / (threads * side));
+  const int64_t resident = (int64_t)sm_count() * 2 * ((nc == 1 ? 1536 : nc == 4 && threads <= 384 ? 1152 : 1024) / (threads * side));
   const int64_t fair = (p.rows * col_blocks + resident - 1) / resident;
   const int most = kSplit ? 16 : p.width >= 4096 ? 8 : p.width <= 1024 ? 32 : 32768 / p.width;
   const int block_rows = (int)(fair < most ? fair : most);
@@ -702,13 +702,14 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)((p.rows + turns * side - 1) / (turns * side)), (unsigned)col_blocks);
   const dim3 block((unsigned)threads, (unsigned)side);
   const size_t smem = BLOCK ? (size_t)nc * threads * 8 / p.block * turns * side : 0;
-#define ROW(NC) row_quant_kernel<OP, BF16, VEC, BLOCK, NC><<<grid, block, smem, stream>>>(p, turns)
-  if (nc == 1) ROW(1);
+#define ROW(NC, THREADS) row_quant_kernel<OP, BF16, VEC, BLOCK, NC, THREADS><<<grid, block, smem, stream>>>(p, turns)
+  if (nc == 1) ROW(1, 256);
   if constexpr (!kSplit) {
-    if (nc == 2) ROW(2);
-    if (nc == 4) ROW(4);
+    if (nc == 2) ROW(2, 512);
+    if (nc == 4 && threads <= 384) ROW(4, 384);
+    if (nc == 4 && threads > 384) ROW(4, 1024);
     if constexpr (OP != OP_NORM)
-      if (nc == 0) ROW(0);
+      if (nc == 0) ROW(0, 1024);
   }
 #undef ROW
   CUDA_TRY(cudaGetLastError());
