@@ -339,7 +339,19 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   const int n0 = blockIdx.y * 128, t0 = blockIdx.z * NT;
   const int ks0 = p.k_stages * rank / S, ks1 = p.k_stages * (rank + 1) / S;
 
-  if (threadIdx.x == 0) {
+  // warp 0: one thread feeds the ring; the first round of loads does not wait for the rest of the block
+  int ks = ks0, stage = 0;
+  uint32_t phase = 0;
+  auto load = [&]() {
+    mbar_expect_tx(bar_full + 8 * stage, F::kStageBytes);
+    const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
+    tma_load_2d(sw, &tm_w, ks * kStageK, n0, bar_full + 8 * stage);
+    tma_load_2d(sw + kTile, &tm_x, ks * kStageK, t0, bar_full + 8 * stage);
+    if (++stage == kStages) { stage = 0; phase ^= 1; }
+    ++ks;
+  };
+  const bool feeder = warp == 0 && elect_one();
+  if (feeder) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
@@ -347,11 +359,10 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     mbar_init(bar_done, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+    while (ks < ks1 && ks - ks0 < kStages) load();
   }
-  if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tm_w);
-    prefetch_tmap(&tm_x);
-  }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_holder), F::kTmemCols);
     tmem_relinquish();
@@ -362,17 +373,8 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   const uint32_t tmem_base = *tmem_holder;
 
   if (warp == 0) {
-    if (elect_one()) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int ks = ks0; ks < ks1; ++ks) {
-        if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status)) break;
-        mbar_expect_tx(bar_full + 8 * stage, F::kStageBytes);
-        const uint32_t sw = smem_u32(smem + stage * F::kStageBytes);
-        tma_load_2d(sw, &tm_w, ks * kStageK, n0, bar_full + 8 * stage);
-        tma_load_2d(sw + kTile, &tm_x, ks * kStageK, t0, bar_full + 8 * stage);
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
-      }
+    if (feeder) {
+      while (ks < ks1 && mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status)) load();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -401,7 +403,14 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   const int tokens = min(NT, p.M - t0);
   int* part = reinterpret_cast<int*>(smem);       // every load and MMA is done by then
   bool live = true;
+  const int n = n0 + lane * 4;
+  float s_b[4], bias[4];
   if (warp >= 2) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s_b[k] = n + k < p.N ? __ldg(p.s_b + n + k) : 0.f;
+      bias[k] = n + k < p.N && p.bias ? __ldg(p.bias + n + k) : 0.f;
+    }
     live = epi_all(mbar_wait(bar_done, 0, abort_flag, p.status));
     if (live) {
       tc_fence_after();
@@ -420,13 +429,6 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   if constexpr (S > 1) cluster_sync_all();
   else if (warp >= 2) epi_bar_sync();
   if (warp >= 2 && live) {
-    const int n = n0 + lane * 4;
-    float s_b[4], bias[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s_b[k] = n + k < p.N ? __ldg(p.s_b + n + k) : 0.f;
-      bias[k] = n + k < p.N && p.bias ? __ldg(p.bias + n + k) : 0.f;
-    }
     constexpr int kBatch = S >= 8 ? 2 : 16 / S > 8 ? 8 : 16 / S;     // tokens whose sums are on their way at once
     const uint32_t mine = smem_u32(part) + lane * 16;
     for (int t = rank + S * (warp - 2); t < tokens; t += 4 * S * kBatch) {
