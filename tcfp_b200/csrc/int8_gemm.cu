@@ -143,6 +143,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   cluster_sync_all();   // both CTAs' barriers exist before anything remote touches them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  let_next_start();
+  wait_for_stream();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -351,7 +353,10 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     ++ks;
   };
   const bool feeder = warp == 0 && elect_one();
+  let_next_start();
   if (feeder) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
@@ -360,6 +365,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
+    wait_for_stream();
     while (ks < ks1 && ks - ks0 < kStages) load();
   }
   __syncwarp();
@@ -406,6 +412,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   const int n = n0 + lane * 4;
   float s_b[4], bias[4];
   if (warp >= 2) {
+    wait_for_stream();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       s_b[k] = n + k < p.N ? __ldg(p.s_b + n + k) : 0.f;
@@ -567,11 +574,12 @@ int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {2, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  allow_early_start(cfg);
   CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_pair_kernel<OUT_BF16>, tm_a, tm_b, tm_out, p, tma_store));
   return TCFP_OK;
 }
@@ -589,11 +597,12 @@ int launch_few(const Operands& o, const Int8Params& p, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = Few<NT>::smem(p.stages);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {S, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  allow_early_start(cfg);
   CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_few_kernel<NT, S>, tm_w, tm_x, p));
   return TCFP_OK;
 }

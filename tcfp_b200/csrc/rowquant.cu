@@ -293,6 +293,8 @@ row_quant_kernel(const RowParams p, const int turns) {
   using E = Elem<BF16>;
   constexpr int kHeld = NC ? NC : 1;
   constexpr bool AHEAD = NC == 1 || NC == 2;
+  let_next_start();
+  wait_for_stream();
   const int step = blockDim.x, span = 8 * step, side = blockDim.y;
   const int col0 = kHeld * span * (int)blockIdx.y;
   const int first = (VEC ? 8 : 1) * (int)threadIdx.x + col0;
@@ -405,6 +407,8 @@ row_quant_kernel(const RowParams p, const int turns) {
 template <int OP, int CH>
 __global__ void __launch_bounds__(256, 3) row_int8_kernel(const RowParams p) {
   __shared__ __align__(16) float s_sum[8], s_max[8];
+  let_next_start();
+  wait_for_stream();
   const int step = blockDim.x, span = 8 * step;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= p.rows) return;      // a whole warp: more than a warp a row has the block to itself
@@ -493,6 +497,8 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_kernel(const NormBwdPa
   extern __shared__ float s_acc[];       // (rows side by side, 8, threads of a row)
   using E = Elem<BF16>;
   const int step = blockDim.x, side = blockDim.y;
+  let_next_start();
+  wait_for_stream();
   const int i0 = (VEC ? 8 : 1) * (int)threadIdx.x, left = p.width - i0;
   const int tid = threadIdx.y * step + threadIdx.x;
   if (tid < 64) slots.v[0][tid] = slots.v[1][tid] = 0.f;
@@ -557,6 +563,8 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_wide_kernel(const Norm
   const int step = blockDim.x, span = 8 * step;
   const int first = (VEC ? 8 : 1) * (int)threadIdx.x;
   const int chunks = (p.width + span - 1) / span;
+  let_next_start();
+  wait_for_stream();
   for (int k = 0; k < 8 * chunks; ++k) s_acc[k * step + threadIdx.x] = 0.f;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
@@ -600,6 +608,8 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_wide_kernel(const Norm
 // out[c] = sum over r of partial[r, c]; 32 columns a block, the rows dealt to 16 warps and joined in a fixed order
 __global__ void column_sum_kernel(const float* __restrict__ partial, int rows, int width, float* __restrict__ out) {
   __shared__ float s[16][32];
+  let_next_start();
+  wait_for_stream();
   const int c = blockIdx.x * 32 + threadIdx.x;
   float t = 0.f;
   if (c < width) {
@@ -628,6 +638,8 @@ struct GateBwdParams {
 // sigma = 1/(1+e^-g): dgate = dy * u * sigma * (1 + g (1 - sigma)), dup = dy * g * sigma
 template <bool BF16, bool VEC>
 __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
+  let_next_start();
+  wait_for_stream();
   const int step = blockDim.x;
   const int i0 = (VEC ? 8 : 1) * (int)threadIdx.x + 8 * step * (int)blockIdx.y;
   const int64_t row = blockIdx.x;
@@ -674,9 +686,8 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
     if (units > 32 && units <= 1024 && p.rows >= 16 * (int64_t)sm_count()) {
       const int threads = units <= 128 ? 32 : round32((units + 3) / 4), side = threads == 32 ? 4 : 1;
       const unsigned blocks = (unsigned)((p.rows + side - 1) / side);
-      if (units <= 64) row_int8_kernel<OP, 2><<<blocks, dim3(threads, side), 0, stream>>>(p);
-      else row_int8_kernel<OP, 4><<<blocks, dim3(threads, side), 0, stream>>>(p);
-      CUDA_TRY(cudaGetLastError());
+      if (units <= 64) CUDA_TRY(launch_early(row_int8_kernel<OP, 2>, dim3(blocks), dim3(threads, side), 0, stream, p));
+      else CUDA_TRY(launch_early(row_int8_kernel<OP, 4>, dim3(blocks), dim3(threads, side), 0, stream, p));
       return TCFP_OK;
     }
   }
@@ -702,7 +713,7 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)((p.rows + turns * side - 1) / (turns * side)), (unsigned)col_blocks);
   const dim3 block((unsigned)threads, (unsigned)side);
   const size_t smem = BLOCK ? (size_t)nc * threads * 8 / p.block * turns * side : 0;
-#define ROW(NC, THREADS) row_quant_kernel<OP, BF16, VEC, BLOCK, NC, THREADS><<<grid, block, smem, stream>>>(p, turns)
+#define ROW(NC, THREADS) CUDA_TRY(launch_early(row_quant_kernel<OP, BF16, VEC, BLOCK, NC, THREADS>, grid, block, smem, stream, p, turns))
   if (nc == 1) ROW(1, 256);
   if constexpr (!kSplit) {
     if (nc == 2) ROW(2, 512);
@@ -712,7 +723,6 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
       if (nc == 0) ROW(0, 1024);
   }
 #undef ROW
-  CUDA_TRY(cudaGetLastError());
   return TCFP_OK;
 }
 
@@ -768,7 +778,7 @@ template <bool BF16, bool VEC>
 int launch_norm_bwd(const NormBwdParams& p, const NormBwdShape& s, cudaStream_t stream) {
   if (p.width <= kNormBwdWidth) {
     const size_t smem = s.side > 1 ? (size_t)s.side * s.threads * 8 * sizeof(float) : 0;
-    rms_norm_backward_kernel<BF16, VEC><<<s.blocks, dim3(s.threads, s.side), smem, stream>>>(p);
+    CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
   } else {
     const int smem = (p.width + 8191) / 8192 * 8192 * (int)sizeof(float);
     static bool done[64] = {false};
@@ -780,9 +790,8 @@ int launch_norm_bwd(const NormBwdParams& p, const NormBwdShape& s, cudaStream_t 
                                     kMaxNormWidth * (int)sizeof(float)));
       done[dev] = true;
     }
-    rms_norm_backward_wide_kernel<BF16, VEC><<<s.blocks, s.threads, smem, stream>>>(p);
+    CUDA_TRY(launch_early(rms_norm_backward_wide_kernel<BF16, VEC>, dim3(s.blocks), dim3(s.threads), smem, stream, p));
   }
-  CUDA_TRY(cudaGetLastError());
   return TCFP_OK;
 }
 
@@ -855,8 +864,7 @@ extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const v
   if (dtype == TCFP_BF16) rc = vec ? launch_norm_bwd<true, true>(p, shape, stream) : launch_norm_bwd<true, false>(p, shape, stream);
   else rc = vec ? launch_norm_bwd<false, true>(p, shape, stream) : launch_norm_bwd<false, false>(p, shape, stream);
   if (rc != TCFP_OK || blocks == 1) return rc;
-  column_sum_kernel<<<(unsigned)((width + 31) / 32), dim3(32, 16), 0, stream>>>(p.dw, blocks, (int)width, dw);
-  CUDA_TRY(cudaGetLastError());
+  CUDA_TRY(launch_early(column_sum_kernel, dim3((unsigned)((width + 31) / 32)), dim3(32, 16), 0, stream, p.dw, blocks, (int)width, dw));
   return TCFP_OK;
 }
 
@@ -877,12 +885,11 @@ extern "C" int32_t tcfp_silu_mul_backward(const void* dy, int64_t ld_dy, const v
   const int threads = units < 256 ? round32(units) : 256;
   const dim3 grid((unsigned)rows, (unsigned)((units + threads - 1) / threads));
   if (dtype == TCFP_BF16) {
-    if (vec) silu_mul_backward_kernel<true, true><<<grid, threads, 0, stream>>>(p);
-    else silu_mul_backward_kernel<true, false><<<grid, threads, 0, stream>>>(p);
+    if (vec) CUDA_TRY(launch_early(silu_mul_backward_kernel<true, true>, grid, dim3(threads), 0, stream, p));
+    else CUDA_TRY(launch_early(silu_mul_backward_kernel<true, false>, grid, dim3(threads), 0, stream, p));
   } else {
-    if (vec) silu_mul_backward_kernel<false, true><<<grid, threads, 0, stream>>>(p);
-    else silu_mul_backward_kernel<false, false><<<grid, threads, 0, stream>>>(p);
+    if (vec) CUDA_TRY(launch_early(silu_mul_backward_kernel<false, true>, grid, dim3(threads), 0, stream, p));
+    else CUDA_TRY(launch_early(silu_mul_backward_kernel<false, false>, grid, dim3(threads), 0, stream, p));
   }
-  CUDA_TRY(cudaGetLastError());
   return TCFP_OK;
 }
