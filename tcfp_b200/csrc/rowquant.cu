@@ -154,9 +154,15 @@ __device__ __forceinline__ float row_reduce(float v, float* slots) {
 }
 
 // ---- the operators ------------------------------------------------------------------
-// silu(g) * u.  __expf and the fast division are good to a few units in the last place of 32 bits (and give the
-// limits 0 and g for large |g|); the result is rounded to 8 bits.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// sigma(g) = 1 / (1 + 2^(-g log2 e)) by the approximate instructions that flush what is below 2^-126: good to about |g| + 8
+// units of 2^-24 (the product's rounding becomes the exponent's error), with the limits 0 and 1 for large |g|.
+__device__ __forceinline__ float sigmoid(float g) {
+  float t, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
+  return r;
+}
+__device__ __forceinline__ float gated(float g, float u) { return g * sigmoid(g) * u; }
 
 // eight values of the one or two inputs of a row
 template <int OP, bool BF16, bool VEC>
@@ -230,8 +236,12 @@ __device__ __forceinline__ int store_block(const float (&v)[8], uint8_t* codes, 
   am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 2));
   if (block >= 64) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 4));
   if (block == 128) am = fmaxf(am, __shfl_xor_sync(0xFFFFFFFFu, am, 8));
-  const int e = block_exponent_fast<false>(am);
-  // -126 <= e <= 120: both powers are normal numbers
+  // the rule of block_exponent(): ceil(log2(am / 448)) with 448 = 1.75 * 2^8, so one is added from a mantissa of 1.75 on; the
+  // 256 numbers there take the full rule.  am >= 1e-12, so -48 <= e <= 120 and both powers are normal numbers
+  am = fmaxf(am, kAmaxFloor);
+  const uint32_t up = __float_as_uint(am) + 0x200000u;
+  int e = (int)(up >> 23) - 127 - 8;
+  if ((up & 0x7FFFFFu) < 256u) e = block_exponent(am, kE4M3Max);
   const float fwd = __uint_as_float((uint32_t)(127 - e) << 23), inv = __uint_as_float((uint32_t)(127 + e) << 23);
   uint32_t pc[4];
 #pragma unroll
@@ -649,7 +659,7 @@ __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
   load8<BF16, VEC>(u, p.up, row * p.ld_up + i0, p.width - i0, step);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float sig = __fdividef(1.f, 1.f + __expf(-g[j]));
+    const float sig = sigmoid(g[j]);
     const float ds = d[j] * sig;
     const float dg = ds * u[j] * fmaf(g[j], 1.f - sig, 1.f);
     u[j] = ds * g[j];

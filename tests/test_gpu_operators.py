@@ -8,9 +8,10 @@ E4M3 round by at most 2^-8 and 2^-4 of the value (E4M3 below 2^-6: by 2^-10).
 * norm: a thread adds at most 32 squares, at most 10 tree steps follow, and
   the division, the addition of eps and rsqrtf (2 ulp = 4u) join: rstd is off by
   at most (32 + 10 + 2 + 4) u / 2 + 4u < 32 u, y by two more roundings: Y = 40 u.
-* gate: __expf is off by 2 + 1.18 |g| ulp, __fdividef by 2 ulp; with |g| <= 40
-  y = g * sigma * u is off by at most (50 + 2 + 2) ulp = 108 u of itself: G = 128 u.
-  Where 1 + e^-g passes 2^126 the fast division returns 0, for a value below
+* gate: the product -g log2 e is off by 2 u of itself, 2 |g| u of the power of
+  two; that instruction adds 2^-22, the addition u, the reciprocal 2 u, two
+  products 2 u; with |g| <= 40 y = g * sigma * u is off by at most 89 u of itself:
+  G = 128 u.  Where 1 + e^-g passes 2^126 the reciprocal is 0, for a value below
   |u| * 88 * 2^-126.
 * a code of step s is off by s / 2 and by what y is off.
 """
