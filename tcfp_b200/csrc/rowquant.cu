@@ -501,33 +501,40 @@ struct NormBwdParams {
 // every gridDim.x-th group of rows, a thread owns the same 8 columns of all its rows, keeps the weight and its part of dw
 // in registers and has the next row on its way while it works on this one.  32768 x 4096 bf16 180 us (5.96 TB/s, the column
 // sums included); without the row ahead 249 us.
-template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(1024) rms_norm_backward_kernel(const NormBwdParams p) {
+template <bool BF16, bool VEC, int CH>
+__global__ void __launch_bounds__(CH == 1 ? 1024 : 512) rms_norm_backward_kernel(const NormBwdParams p) {
   __shared__ __align__(16) Slots slots;
-  extern __shared__ float s_acc[];       // (rows side by side, 8, threads of a row)
+  extern __shared__ float s_acc[];       // (rows side by side, 8 * CH, threads of a row)
   using E = Elem<BF16>;
-  const int step = blockDim.x, side = blockDim.y;
+  const int step = blockDim.x, span = 8 * step, side = blockDim.y;
   let_next_start();
   wait_for_stream();
-  const int i0 = (VEC ? 8 : 1) * (int)threadIdx.x, left = p.width - i0;
+  const int first = (VEC ? 8 : 1) * (int)threadIdx.x;
   const int tid = threadIdx.y * step + threadIdx.x;
   if (tid < 64) slots.v[0][tid] = slots.v[1][tid] = 0.f;
   __syncthreads();
-  float w[8], acc[8];
-  if (p.w_bf16) load8<true, VEC>(w, p.w, i0, left, step);
-  else load8<false, VEC>(w, p.w, i0, left, step);
+  float w[CH][8], acc[CH][8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  for (int c = 0; c < CH; ++c) {
+    if (p.w_bf16) load8<true, VEC>(w[c], p.w, first + c * span, p.width - first - c * span, step);
+    else load8<false, VEC>(w[c], p.w, first + c * span, p.width - first - c * span, step);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[c][j] = 0.f;
+  }
 
-  Raw<BF16, VEC> dy, h, dh;
+  Raw<BF16, VEC> dy[CH], h[CH], dh[CH];
   float rstd;
   // a row behind the last one is taken as zeros: it adds nothing
   auto load = [&](int64_t row) {
-    const int n = row < p.rows ? left : 0;
-    dy.load(reinterpret_cast<const E*>(p.dy) + row * p.ld_dy + i0, n, step);
-    h.load(reinterpret_cast<const E*>(p.h) + row * p.ld_h + i0, n, step);
-    dh.load(reinterpret_cast<const E*>(p.dh) + row * p.ld_dh + i0, p.dh != nullptr ? n : 0, step);
-    rstd = row < p.rows ? __ldg(p.rstd + row) : 0.f;
+    const bool there = row < p.rows;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = first + c * span, n = there ? p.width - at : 0;
+      dy[c].load(reinterpret_cast<const E*>(p.dy) + row * p.ld_dy + at, n, step);
+      h[c].load(reinterpret_cast<const E*>(p.h) + row * p.ld_h + at, n, step);
+      dh[c].load(reinterpret_cast<const E*>(p.dh) + row * p.ld_dh + at, p.dh != nullptr ? n : 0, step);
+    }
+    rstd = there ? __ldg(p.rstd + row) : 0.f;
   };
   int turn = 0;
   const int64_t stride = (int64_t)gridDim.x * side;
@@ -535,33 +542,43 @@ __global__ void __launch_bounds__(1024) rms_norm_backward_kernel(const NormBwdPa
   load(group + threadIdx.y);
   for (; group < p.rows; group += stride, turn ^= 1) {
     const int64_t row = group + threadIdx.y;
-    float g[8], hat[8];
+    float g[CH][8], hat[CH][8];
+    Raw<BF16, VEC> d[CH];
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      hat[j] = h.get(j) * rstd;
-      acc[j] = fmaf(dy.get(j), hat[j], acc[j]);
-      g[j] = dy.get(j) * w[j];
-      sum = fmaf(g[j], hat[j], sum);
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hat[c][j] = h[c].get(j) * rstd;
+        acc[c][j] = fmaf(dy[c].get(j), hat[c][j], acc[c][j]);
+        g[c][j] = dy[c].get(j) * w[c][j];
+        sum = fmaf(g[c][j], hat[c][j], sum);
+      }
+      d[c] = dh[c];
     }
-    const Raw<BF16, VEC> d = dh;
     const float r = rstd;
     load(row + stride);
     const float mean = row_reduce<false>(sum, slots.v[turn]) * p.inv_width;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = fmaf(r, g[j] - hat[j] * mean, d.get(j));
-    if (row < p.rows) store8<BF16, VEC>(g, p.dx, row * (int64_t)p.width + i0, left, step);
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[c][j] = fmaf(r, g[c][j] - hat[c][j] * mean, d[c].get(j));
+      const int at = first + c * span;
+      if (row < p.rows) store8<BF16, VEC>(g[c], p.dx, row * (int64_t)p.width + at, p.width - at, step);
+    }
   }
   if (side > 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s_acc[(threadIdx.y * 8 + j) * step + threadIdx.x] = acc[j];
+    for (int k = 0; k < 8 * CH; ++k) s_acc[(threadIdx.y * 8 * CH + k) * step + threadIdx.x] = acc[k / 8][k % 8];
     __syncthreads();
     if (threadIdx.y != 0) return;
     for (int y = 1; y < side; ++y)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += s_acc[(y * 8 + j) * step + threadIdx.x];
+      for (int k = 0; k < 8 * CH; ++k) acc[k / 8][k % 8] += s_acc[(y * 8 * CH + k) * step + threadIdx.x];
   }
-  store8<false, VEC>(acc, p.dw, (int64_t)blockIdx.x * p.width + i0, left, step);
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    store8<false, VEC>(acc[c], p.dw, (int64_t)blockIdx.x * p.width + first + c * span, p.width - first - c * span, step);
 }
 
 // The same for rows of more than 8192 values: a block's rows are read twice, the second time from L2, and its part of dw
@@ -771,15 +788,16 @@ constexpr int kNormBwdWidth = 8192;      // 8 values for each of 1024 threads
 
 // threads of a row, rows side by side and blocks of the norm's backward pass: one set of resident blocks
 struct NormBwdShape {
-  int threads, side, blocks;
+  int chunks, threads, side, blocks;
 };
-NormBwdShape norm_bwd_shape(int64_t rows, int64_t width) {
+NormBwdShape norm_bwd_shape(int64_t rows, int64_t width, bool two) {
   const int units = (int)((width + 7) / 8);
   NormBwdShape s;
-  s.threads = units > 1024 ? 1024 : units <= 16 ? 16 : round32(units);
+  s.chunks = two && units > 32 && units <= 1024 ? 2 : 1;
+  s.threads = units > 1024 ? 1024 : units <= 16 ? 16 : round32((units + s.chunks - 1) / s.chunks);
   s.side = s.threads < 256 ? 256 / s.threads : 1;
   const int64_t groups = (rows + s.side - 1) / s.side;
-  const int64_t resident = (int64_t)sm_count() * (width > kNormBwdWidth ? 1 : 1024 / (s.threads * s.side));
+  const int64_t resident = (int64_t)sm_count() * (width > kNormBwdWidth ? 1 : (s.chunks == 2 ? 512 : 1024) / (s.threads * s.side));
   s.blocks = (int)(groups < resident ? groups : resident);
   return s;
 }
@@ -787,8 +805,14 @@ NormBwdShape norm_bwd_shape(int64_t rows, int64_t width) {
 template <bool BF16, bool VEC>
 int launch_norm_bwd(const NormBwdParams& p, const NormBwdShape& s, cudaStream_t stream) {
   if (p.width <= kNormBwdWidth) {
-    const size_t smem = s.side > 1 ? (size_t)s.side * s.threads * 8 * sizeof(float) : 0;
-    CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
+    const size_t smem = s.side > 1 ? (size_t)s.side * s.threads * 8 * s.chunks * sizeof(float) : 0;
+    if constexpr (BF16 && VEC) {
+      if (s.chunks == 2) {
+        CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 2>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
+        return TCFP_OK;
+      }
+    }
+    CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 1>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
   } else {
     const int smem = (p.width + 8191) / 8192 * 8192 * (int)sizeof(float);
     static bool done[64] = {false};
@@ -850,7 +874,7 @@ extern "C" int32_t tcfp_int8_quantize_rows(const void* x, int64_t ld_x, int32_t 
 
 extern "C" size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
   if (rows < 1 || width < 1 || width > kMaxNormWidth) return 0;
-  return (size_t)norm_bwd_shape(rows, width).blocks * (size_t)width * sizeof(float);
+  return (size_t)norm_bwd_shape(rows, width, false).blocks * (size_t)width * sizeof(float);      // never fewer than with two chunks
 }
 
 extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h, int64_t ld_h, const float* rstd,
@@ -864,12 +888,12 @@ extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const v
   if (rows < 1 || width < 1) return fail(TCFP_ERR_INVALID, "%s: %lld rows, width %lld", what, (long long)rows, (long long)width);
   if (width > kMaxNormWidth) return fail(TCFP_ERR_UNSUPPORTED, "%s: width %lld above %d", what, (long long)width, kMaxNormWidth);
   const int e = dtype == TCFP_BF16 ? 2 : 4;
-  const NormBwdShape shape = norm_bwd_shape(rows, width);
+  bool vec = width % 8 == 0 && aligned16(dy, ld_dy, e) && aligned16(h, ld_h, e) && (!dh || aligned16(dh, ld_dh, e)) &&
+             aligned16(weight, 0, 1) && aligned16(dx, 0, 1) && aligned16(dw, 0, 1) && aligned16(workspace, 0, 1);
+  const NormBwdShape shape = norm_bwd_shape(rows, width, vec && dtype == TCFP_BF16);
   const int blocks = shape.blocks;
-  NormBwdParams p{dy, h, dh, ld_dy, ld_h, ld_dh, rstd, weight, w_dtype == TCFP_BF16, dx,
-                  blocks == 1 ? dw : reinterpret_cast<float*>(workspace), rows, (int)width, 1.f / (float)width};
-  const bool vec = width % 8 == 0 && aligned16(dy, ld_dy, e) && aligned16(h, ld_h, e) && (!dh || aligned16(dh, ld_dh, e)) &&
-                   aligned16(weight, 0, 1) && aligned16(dx, 0, 1) && aligned16(p.dw, 0, 1);
+  const NormBwdParams p{dy, h, dh, ld_dy, ld_h, ld_dh, rstd, weight, w_dtype == TCFP_BF16, dx,
+                        blocks == 1 ? dw : reinterpret_cast<float*>(workspace), rows, (int)width, 1.f / (float)width};
   int rc;
   if (dtype == TCFP_BF16) rc = vec ? launch_norm_bwd<true, true>(p, shape, stream) : launch_norm_bwd<true, false>(p, shape, stream);
   else rc = vec ? launch_norm_bwd<false, true>(p, shape, stream) : launch_norm_bwd<false, false>(p, shape, stream);
