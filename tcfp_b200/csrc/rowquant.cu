@@ -498,11 +498,12 @@ struct NormBwdParams {
 
 // dx = rstd * (g - hat * mean(g * hat)) + dh with g = dy * w, hat = h * rstd;  dw = sum over rows of dy * hat.
 // Bound by memory: 6 bytes in and 2 out a bf16 value.  blockDim = (threads of a row, rows side by side); a block walks
-// every gridDim.x-th group of rows, a thread owns the same 8 columns of all its rows, keeps the weight and its part of dw
-// in registers and has the next row on its way while it works on this one.  32768 x 4096 bf16 180 us (5.96 TB/s, the column
-// sums included); without the row ahead 249 us.
-template <bool BF16, bool VEC, int CH>
-__global__ void __launch_bounds__(CH == 1 ? 1024 : 512) rms_norm_backward_kernel(const NormBwdParams p) {
+// every gridDim.x-th group of rows, a thread owns the same 8 * CH columns of all its rows, keeps the weight and its part of dw
+// in registers and has the next row on its way while it works on this one.  32768 x 4096 bf16, the column sums included: 170 us
+// (6.3 TB/s) with 16 values a thread, 178 us with 8 (189 us where the power cap holds the clock down: more instructions a
+// value), 249 us without the row ahead.
+template <bool BF16, bool VEC, int CH, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBwdParams p) {
   __shared__ __align__(16) Slots slots;
   extern __shared__ float s_acc[];       // (rows side by side, 8 * CH, threads of a row)
   using E = Elem<BF16>;
@@ -794,10 +795,11 @@ NormBwdShape norm_bwd_shape(int64_t rows, int64_t width, bool two) {
   const int units = (int)((width + 7) / 8);
   NormBwdShape s;
   s.chunks = two && units > 32 && units <= 1024 ? 2 : 1;
+  // blocks of up to 512 threads have 128 registers a thread: FP32 rows and narrow loads spill with 64
   s.threads = units > 1024 ? 1024 : units <= 16 ? 16 : round32((units + s.chunks - 1) / s.chunks);
   s.side = s.threads < 256 ? 256 / s.threads : 1;
   const int64_t groups = (rows + s.side - 1) / s.side;
-  const int64_t resident = (int64_t)sm_count() * (width > kNormBwdWidth ? 1 : (s.chunks == 2 ? 512 : 1024) / (s.threads * s.side));
+  const int64_t resident = (int64_t)sm_count() * (width > kNormBwdWidth ? 1 : s.threads > 512 ? 1 : 512 / (s.threads * s.side));
   s.blocks = (int)(groups < resident ? groups : resident);
   return s;
 }
@@ -808,11 +810,12 @@ int launch_norm_bwd(const NormBwdParams& p, const NormBwdShape& s, cudaStream_t 
     const size_t smem = s.side > 1 ? (size_t)s.side * s.threads * 8 * s.chunks * sizeof(float) : 0;
     if constexpr (BF16 && VEC) {
       if (s.chunks == 2) {
-        CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 2>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
+        CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 2, 512>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
         return TCFP_OK;
       }
     }
-    CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 1>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
+    if (s.threads <= 512) CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 1, 512>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
+    else CUDA_TRY(launch_early(rms_norm_backward_kernel<BF16, VEC, 1, 1024>, dim3(s.blocks), dim3(s.threads, s.side), smem, stream, p));
   } else {
     const int smem = (p.width + 8191) / 8192 * 8192 * (int)sizeof(float);
     static bool done[64] = {false};
@@ -874,7 +877,9 @@ extern "C" int32_t tcfp_int8_quantize_rows(const void* x, int64_t ld_x, int32_t 
 
 extern "C" size_t tcfp_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
   if (rows < 1 || width < 1 || width > kMaxNormWidth) return 0;
-  return (size_t)norm_bwd_shape(rows, width, false).blocks * (size_t)width * sizeof(float);      // never fewer than with two chunks
+  // the call's alignment, which it does not know, decides between the two shapes
+  const int one = norm_bwd_shape(rows, width, false).blocks, two = norm_bwd_shape(rows, width, true).blocks;
+  return (size_t)(one > two ? one : two) * (size_t)width * sizeof(float);
 }
 
 extern "C" int32_t tcfp_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h, int64_t ld_h, const float* rstd,

@@ -507,3 +507,23 @@ def test_offsets_past_32_bits():
     sa, sb = torch.rand(m, generator=gen(63)).to(DEV), torch.rand(n, generator=gen(64)).to(DEV)
     out = K.int8_matmul(a, b, sa, sb, out_dtype=torch.bfloat16)
     assert torch.equal(out[-300:], K.int8_matmul(a[-300:], b, sa[-300:], sb, out_dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [40, 264, 1000, 1001, 2048, 4096, 8192, 9000])
+def test_norm_backward_keeps_inside_its_workspace(width, dtype):
+    """Not a byte behind tcfp_rms_norm_backward_workspace_bytes() is written, whichever shape the call takes."""
+    from tcfp_b200 import _C
+
+    lib = _C.load()
+    for rows in (1, 300, 5000):
+        x = stream(70, rows, width, dtype)
+        w, rstd = torch.ones(width, device=DEV), torch.ones(rows, device=DEV)
+        n = lib.tcfp_rms_norm_backward_workspace_bytes(rows, width)
+        guard = 4 * width * 600                       # a margin larger than any other shape's workspace
+        ws = torch.full((n + guard,), 113, dtype=torch.uint8, device=DEV)
+        dx, dw = torch.empty_like(x), torch.empty(width, device=DEV)
+        _C.check(lib.tcfp_rms_norm_backward(x.data_ptr(), width, x.data_ptr(), width, rstd.data_ptr(), _C.dtype_code(x),
+                                            w.data_ptr(), _C.F32, None, 0, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), rows,
+                                            width, _C.stream()))
+        assert (ws[n:] == 113).all()
