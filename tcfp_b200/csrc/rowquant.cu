@@ -296,7 +296,7 @@ __device__ __forceinline__ void flush_exponents(const int8_t* s_e, const RowPara
 // blockDim.y places.  gridDim.y > 1 (only where no statistic spans the row) splits the row's columns.  NC = 0 walks a
 // row of any width and loads it again for each pass.
 template <int OP, bool BF16, bool VEC, bool BLOCK, int NC, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 6 : THREADS == 384 ? 3 : THREADS == 512 ? 2 : 1)
+__global__ void __launch_bounds__(THREADS, !VEC && OP == OP_NORM ? 1 : THREADS == 256 ? 6 : THREADS == 384 ? 3 : THREADS == 512 ? 2 : 1)
 row_quant_kernel(const RowParams p, const int turns) {
   __shared__ __align__(16) Slots s_sum, s_max;
   extern __shared__ int8_t s_e[];
@@ -698,13 +698,14 @@ int round32(int x) { return (x + 31) & ~31; }
 
 int block_shift(int block) { return block == 128 ? 7 : block == 64 ? 6 : 5; }
 
-// Threads and values a thread (8 * NC), by the row's width, and rows a block.  Measured at 32768 x 4096 bf16, block 64,
-// with a residual: 256 threads x 16 values with the next row on its way 149 us (6.30 TB/s), without 172 us; 128 threads x
-// 32 values 215 us; 8 rows a block 149 us, 16 rows 155 us, 1 row 230 us (nothing ahead, and the exponents leave as single
-// bytes).  Narrower rows want more of them: 16384 x 1024 27 us with 8 rows, 24 us with 16.  A row of more than 8192 values
-// takes 32 a thread and no load ahead (registers).  The gated block form has no row statistic: 128 threads x 8 values
-// walk 16 rows of 1024 columns, 16384 x 11008 170 us (5.3 TB/s), 256 threads 175 us; reading and writing bf16 values too
-// 212 us (5.9 TB/s).
+// Threads and values a thread (8 * NC), by the row's width, and rows a block.  Measured at 32768 x 4096 bf16, block 64, with a
+// residual: 256 threads x 16 values with the next row on its way 149 us (6.3 TB/s), without 172 us; 128 threads x 32 values
+// 215 us; 8 rows a block 149 us, 16 rows 155 us, 1 row 230 us (nothing ahead, and the exponents leave as single bytes).
+// Narrower rows want more of them: 16384 x 1024 27 us with 8 rows, 23 us with 32.  A row of more than 8192 values takes 32 a
+// thread and no load ahead (registers); up to 12288 three blocks share an SM: gate 16384 x 11008 to int8 153 us (5.9 TB/s),
+// two blocks 195 us.  The gated block form has no row statistic: 128 threads x 8 values walk 16 rows of 1024 columns,
+// 16384 x 11008 155 us (5.8 TB/s), with bf16 values 208 us (6.1 TB/s); 256 threads 175 and 234 us (before the shorter sigmoid).
+// Rows off 16-byte boundaries take single values and are bound by their instructions: 16384 x 1001 FP32 norm 49 us (3.7 TB/s).
 template <int OP, bool BF16, bool VEC, bool BLOCK>
 int launch_row(const RowParams& p, cudaStream_t stream) {
   constexpr bool kSplit = OP != OP_NORM && BLOCK;       // the row's columns over several blocks
