@@ -4,7 +4,8 @@ Host side is Python/PyTorch; the compute lives in ``libtcfp_b200.so`` (C ABI in
 ``include/tcfp_b200.h``), built in-tree by ``python -m tcfp_b200.build``.
 Sub-modules: ``core`` (FP8 casts, error-feedback state), ``kernels`` and
 ``cuda_ext`` (launch wrappers under the reference's names), ``nn``
-(``TCFPLinear``, ``convert_to_tcfp``), ``tp`` (tensor parallelism),
+(``TCFPLinear``, ``convert_to_tcfp``; the norm and gated activation that write a
+layer's 8-bit input, ``Int8Linear``), ``tp`` (tensor parallelism),
 ``checkpoint``, ``host_pipeline``, ``workloads``, ``microbench``.
 """
 from . import core as _core
