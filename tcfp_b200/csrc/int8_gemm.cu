@@ -376,6 +376,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  wait_for_stream();      // every role, so that no bounded wait below counts the time of the kernel before this one
   const uint32_t tmem_base = *tmem_holder;
 
   if (warp == 0) {
@@ -412,7 +413,6 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   const int n = n0 + lane * 4;
   float s_b[4], bias[4];
   if (warp >= 2) {
-    wait_for_stream();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       s_b[k] = n + k < p.N ? __ldg(p.s_b + n + k) : 0.f;

@@ -291,10 +291,10 @@ __device__ __forceinline__ void flush_exponents(const int8_t* s_e, const RowPara
 }
 
 // blockDim = (threads of a row, rows side by side).  A thread holds 8 * NC values of its row in registers, and while it
-// works on them the inputs of its next row are on their way (NC 1 and 2; bringing a wider row's next one to shared memory with
-// cp.async measured slower: gate 16384 x 11008 to int8 210 -> 233 us, norm to block codes 308 -> 359 us).  The block walks `turns` rows for each of its
-// blockDim.y places.  gridDim.y > 1 (only where no statistic spans the row) splits the row's columns.  NC = 0 walks a
-// row of any width and loads it again for each pass.
+// works on them the inputs of its next row are on their way (NC 1 and 2; bringing a wider row's next one to shared memory
+// with cp.async measured slower: gate 16384 x 11008 to int8 210 -> 233 us, norm to block codes 308 -> 359 us).  The block
+// walks `turns` rows for each of its blockDim.y places.  gridDim.y > 1 (only where no statistic spans the row) splits the
+// row's columns.  NC = 0 walks a row of any width and loads it again for each pass.
 template <int OP, bool BF16, bool VEC, bool BLOCK, int NC, int THREADS>
 __global__ void __launch_bounds__(THREADS, !VEC && OP == OP_NORM ? 1 : THREADS == 256 ? 6 : THREADS == 384 ? 3 : THREADS == 512 ? 2 : 1)
 row_quant_kernel(const RowParams p, const int turns) {
@@ -413,7 +413,8 @@ row_quant_kernel(const RowParams p, const int turns) {
 // The same for many bf16 rows in int8 (OP_NORM or OP_COPY): one row for each place of a block, 8 * CH values a thread that
 // wait in registers as they came, 2 bytes a value, and are formed again for each of the passes (sum of squares, maximum,
 // codes).  Twice the values a thread halves what a row costs each of them (two reductions, the scale), and many small blocks
-// hide one another's barriers.  32768 x 4096 with a residual 163 us (5.8 TB/s), 178 us in row_quant_kernel; without norm 89 / 96 us.
+// hide one another's barriers.  32768 x 4096 with a residual 141 us (6.65 TB/s), the codes alone 64 us (6.3 TB/s); when both still
+// divided near ties, 163 and 89 us here against 178 and 96 us in row_quant_kernel.
 template <int OP, int CH>
 __global__ void __launch_bounds__(256, 3) row_int8_kernel(const RowParams p) {
   __shared__ __align__(16) float s_sum[8], s_max[8];

@@ -527,3 +527,43 @@ def test_norm_backward_keeps_inside_its_workspace(width, dtype):
                                             w.data_ptr(), _C.F32, None, 0, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), rows,
                                             width, _C.stream()))
         assert (ws[n:] == 113).all()
+
+
+def test_capture_after_copies_memsets_and_joins():
+    """The operators start early only behind another kernel: captured behind a copy, a memset, another library kernel and the
+    join of two streams they replay the eager bytes."""
+    from tcfp_b200 import kernels as K
+
+    rows, d = 200, 512
+    w = torch.ones(d, device=DEV)
+    wq = K.int8_quantize_rows(stream(80, 384, d, torch.float32))
+    src = [stream(81 + i, rows, d, torch.bfloat16) for i in range(3)]
+    x, r = torch.empty_like(src[0]), torch.empty_like(src[0])
+    side = torch.cuda.Stream()
+
+    def step(first, second):
+        x.copy_(first)                                        # copy -> row kernel
+        q0 = K.int8_quantize_rows(x)
+        r.zero_()                                             # memset -> row kernel
+        q1, h, rstd = K.add_rms_norm_quantize(x, w, r)
+        x.add_(second)                                        # library kernel -> product, whose other input came from a row kernel
+        y = K.int8_matmul(q1.codes, wq.codes, q1.scales, wq.scales)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            z = K.int8_matmul(q0.codes, wq.codes, q0.scales, wq.scales)
+        few = K.int8_matmul(q1.codes[:3], wq.codes, q1.scales[:3], wq.scales)
+        torch.cuda.current_stream().wait_stream(side)         # join -> row kernel
+        return y, z, few, *K.add_rms_norm_backward(x, h, rstd, w, x), K.silu_mul_quantize(x).codes
+
+    eager = [[t.clone() for t in step(src[i], src[i + 1])] for i in range(2)]
+    first, second = src[0].clone(), src[1].clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(first, second)
+    for i in (0, 1, 0):
+        first.copy_(src[i])
+        second.copy_(src[i + 1])
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, eager[i]):
+            assert torch.equal(a, b)
