@@ -7,8 +7,8 @@
 //
 //   int8_pair_kernel  prompts: a pair of CTAs (cta_group::2) owns a 256 x 256 output tile, as the FP8 pair kernel does.
 //                     Bound by the tensor pipe: 8192 x 12288 x 4096 252 us, 3.27 Pop/s (98 % of twice the measured bf16
-//                     rate).  The channel scales of a tile wait in shared memory: read from global memory by every
-//                     thread, the epilogue took 7 us a tile and set the pace for K below 2048.
+//                     rate).  The channel scales of a tile wait in shared memory: with every thread reading them from
+//                     global memory the epilogue took 7 us a tile and set the pace for K below 2048.
 //   int8_few_kernel   few tokens: bound by the weight's bytes, so the weight takes the 128 rows of the MMA and the tokens
 //                     its 16..128 columns, and the CTAs of a cluster split K; the partial sums meet through distributed
 //                     shared memory.  Integer sums do not depend on the split.  22016 x 4096: 19 us for 1 to 32 tokens
@@ -61,18 +61,20 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint6
         : "memory");
 }
 
-// whether all 128 epilogue threads got through a wait: they go on or leave together, so that none is missing at a barrier
-__device__ __forceinline__ bool epi_all(bool ok) {
+// whether all 128 threads that share barrier `id` got through a wait: they go on or leave together, so that none is missing
+// at a barrier
+__device__ __forceinline__ bool epi_all(bool ok, int id = 1) {
   uint32_t all;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "bar.red.and.pred p, 1, 128, q;\n\t"
+      "bar.red.and.pred p, %2, 128, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(all)
-      : "r"((uint32_t)ok)
+      : "r"((uint32_t)ok), "r"(id)
       : "memory");
   return all != 0;
 }
+__device__ __forceinline__ void epi_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
 __device__ __forceinline__ float scaled(int acc, float s_a, float s_b, float bias) {
   return fmaf(__int2float_rn(acc) * s_a, s_b, bias);
@@ -87,8 +89,9 @@ constexpr int kPieceBytes = 16384;            // 128 rows x 128 bytes of staged 
 constexpr int kColumnBytes = 2 * 2 * 256 * 4;   // channel scales and bias of two tiles
 constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 2 * kPieceBytes + kColumnBytes + 256;
 
-template <bool OUT_BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+// G groups of four epilogue warps share a tile's columns
+template <bool OUT_BF16, int G>
+__global__ void __launch_bounds__(64 + 128 * G, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                  const __grid_constant__ CUtensorMap tm_out, const Int8Params p, const int tma_store) {
   constexpr int kStages = kPairStages;
@@ -124,7 +127,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_tfull + 8 * b, 1);
-      mbar_init(bar_tempty + 8 * b, 8);   // one arrival per epilogue warp of both CTAs
+      mbar_init(bar_tempty + 8 * b, 8 * G);  // one arrival per epilogue warp of both CTAs
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -195,59 +198,68 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     }
     __syncwarp();
   } else {
-    // epilogue: both CTAs, 128 rows each, 32 accumulator columns at a time
-    constexpr int kPieceCols = OUT_BF16 ? 64 : 32;       // columns in a 128-byte row of the staging buffer
+    // epilogue: both CTAs, 128 rows each; a group takes its columns 32 at a time and has the next ones on their way.  One group
+    // alternates between the two staging pieces, two have one each
+    constexpr int kCols = 256 / G;
+    constexpr int kPieceCols = OUT_BF16 ? 64 : 32;       // columns in a 128-byte row of the staging piece
     constexpr int kElem = OUT_BF16 ? 2 : 4;
+    const int group = G == 2 && warp >= 6, id = 1 + group;
     const int q = warp & 3;
     const int r_local = q * 32 + lane;
-    const bool issuer = threadIdx.x == 64;
-    int buf = 0, sbuf = 0, pending = 0;
+    const bool issuer = threadIdx.x == 64 + 128 * group;
+    uint8_t* piece = staging + group * kPieceBytes;
+    int buf = 0;
     uint32_t buf_phase = 0;
     for (int tile = pair; tile < num_tiles; tile += num_pairs) {
       int mb, nb;
       coords(tile, mb, nb);
-      const int row0 = mb * 256 + (int)rank * 128;
+      const int row0 = mb * 256 + (int)rank * 128, col0 = nb * 256 + group * kCols;
       const float s_a = row0 + r_local < p.M ? __ldg(p.s_a + row0 + r_local) : 0.f;
-      // this tile's channel scales and bias; the tile before may still be read from the other half
-      float* s_col = columns + buf * 512;
-      for (int c = threadIdx.x - 64; c < 256; c += 128) {
-        const int n = nb * 256 + c;
+      // these columns' scales and bias; those of the tile before may still be read from the other buffer
+      float* s_col = columns + (buf * G + group) * 2 * kCols;
+      for (int c = (threadIdx.x - 64) & 127; c < kCols; c += 128) {
+        const int n = col0 + c;
         s_col[c] = n < p.N ? __ldg(p.s_b + n) : 0.f;
-        s_col[256 + c] = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
+        s_col[kCols + c] = n < p.N && p.bias ? __ldg(p.bias + n) : 0.f;
       }
-      if (!epi_all(mbar_wait(bar_tfull + 8 * buf, buf_phase, abort_flag, p.status))) break;
+      if (!epi_all(mbar_wait(bar_tfull + 8 * buf, buf_phase, abort_flag, p.status), id)) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256);
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * 256 + group * kCols);
+      uint32_t v[32];
+      tmem_ld32(t_row, v);
 #pragma unroll 1
-      for (int g = 0; g < 8; ++g) {
-        uint32_t v[32];
-        tmem_ld32(t_row + g * 32, v);
+      for (int g = 0; g < kCols / 32; ++g) {
         tmem_ld_wait();
-        if (g == 7) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa(bar_tempty + 8 * buf, 0));
-        }
         float o[32];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const float4 sb = reinterpret_cast<const float4*>(s_col + g * 32)[c];
-          const float4 bi = reinterpret_cast<const float4*>(s_col + 256 + g * 32)[c];
+          const float4 bi = reinterpret_cast<const float4*>(s_col + kCols + g * 32)[c];
           o[4 * c] = scaled((int)v[4 * c], s_a, sb.x, bi.x);
           o[4 * c + 1] = scaled((int)v[4 * c + 1], s_a, sb.y, bi.y);
           o[4 * c + 2] = scaled((int)v[4 * c + 2], s_a, sb.z, bi.z);
           o[4 * c + 3] = scaled((int)v[4 * c + 3], s_a, sb.w, bi.w);
         }
-        // a staging buffer may be rewritten once the store issued two pieces ago has read it
-        if (!OUT_BF16 || (g & 1) == 0) {
-          if (issuer && pending >= 2) { bulk_wait_read1(); pending = 1; }
-          epi_bar_sync();
+        if (g < kCols / 32 - 1) {
+          tmem_ld32(t_row + (g + 1) * 32, v);       // on its way while this piece is written
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa(bar_tempty + 8 * buf, 0));
         }
-        uint8_t* piece = staging + sbuf * kPieceBytes + r_local * 128;
+        // a piece may be rewritten once the store that last used it has read it
+        if (!OUT_BF16 || (g & 1) == 0) {
+          if (issuer) {
+            if constexpr (G == 1) bulk_wait_read1();
+            else bulk_wait_read0();
+          }
+          epi_sync(id);
+        }
+        uint8_t* line = piece + r_local * 128;
         if constexpr (!OUT_BF16) {
 #pragma unroll
           for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(piece + ((c ^ (r_local & 7)) << 4)) =
+            *reinterpret_cast<float4*>(line + ((c ^ (r_local & 7)) << 4)) =
                 make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
         } else {
 #pragma unroll
@@ -258,33 +270,35 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * c + 2 * k], o[8 * c + 2 * k + 1]);
               w[k] = *reinterpret_cast<uint32_t*>(&b);
             }
-            *reinterpret_cast<uint4*>(piece + ((((g & 1) * 4 + c) ^ (r_local & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(line + ((((g & 1) * 4 + c) ^ (r_local & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         if (OUT_BF16 && (g & 1) == 0) continue;
-        const int nst = nb * 256 + (OUT_BF16 ? (g >> 1) : g) * kPieceCols;
+        const int nst = col0 + (OUT_BF16 ? (g >> 1) : g) * kPieceCols;
         if (tma_store) {
           fence_async_smem();
-          epi_bar_sync();
+          epi_sync(id);
           if (issuer && nst < p.N && row0 < p.M) {
-            tma_store_2d(&tm_out, smem_u32(staging + sbuf * kPieceBytes), nst, row0);
+            tma_store_2d(&tm_out, smem_u32(piece), nst, row0);
             bulk_commit();
-            ++pending;
           }
         } else {
           // rows of out that do not start on 16-byte boundaries: a warp writes a row's piece, neighbouring lanes neighbouring
           // columns
-          epi_bar_sync();
+          epi_sync(id);
           const int rows = min(128, p.M - row0), cols = min(kPieceCols, p.N - nst);
-          for (int r = warp - 2; r < rows; r += 4)
-            for (int c = lane; c < cols; c += 32) {
-              const uint8_t* src = staging + sbuf * kPieceBytes + r * 128 + (((c * kElem >> 4) ^ (r & 7)) << 4) + (c * kElem & 15);
-              const int64_t at = (int64_t)(row0 + r) * p.N + nst + c;
-              if constexpr (OUT_BF16) reinterpret_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(src);
-              else reinterpret_cast<uint32_t*>(p.out)[at] = *reinterpret_cast<const uint32_t*>(src);
-            }
+#pragma unroll 4
+          for (int r = q; r < rows; r += 4)
+#pragma unroll
+            for (int c = lane; c < kPieceCols; c += 32)
+              if (c < cols) {
+                const uint8_t* src = piece + r * 128 + (((c * kElem >> 4) ^ (r & 7)) << 4) + (c * kElem & 15);
+                const int64_t at = (int64_t)(row0 + r) * p.N + nst + c;
+                if constexpr (OUT_BF16) reinterpret_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+                else reinterpret_cast<uint32_t*>(p.out)[at] = *reinterpret_cast<const uint32_t*>(src);
+              }
         }
-        sbuf ^= 1;
+        if constexpr (G == 1) piece = staging + (piece == staging ? kPieceBytes : 0);
       }
       if (++buf == 2) { buf = 0; buf_phase ^= 1; }
     }
@@ -551,7 +565,7 @@ struct Operands {
   int64_t lda, ldb;
 };
 
-template <bool OUT_BF16>
+template <bool OUT_BF16, int G>
 int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
   constexpr int kElem = OUT_BF16 ? 2 : 4;
   CUtensorMap tm_a, tm_b, tm_out;
@@ -565,13 +579,13 @@ int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
                                   p.out, p.M, p.N, pitch, 128)) != TCFP_OK)
     return rc;
   static bool done[64] = {false};
-  if ((rc = allow_smem(int8_pair_kernel<OUT_BF16>, kPairSmem, done)) != TCFP_OK) return rc;
+  if ((rc = allow_smem(int8_pair_kernel<OUT_BF16, G>, kPairSmem, done)) != TCFP_OK) return rc;
   p.group_m = 16;
   const int64_t tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
   const int max_pairs = gemm_sm_budget() / 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * (tiles < max_pairs ? tiles : max_pairs)), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(64 + 128 * G, 1, 1);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -580,7 +594,7 @@ int launch_pair(const Operands& o, Int8Params p, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   allow_early_start(cfg);
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_pair_kernel<OUT_BF16>, tm_a, tm_b, tm_out, p, tma_store));
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, int8_pair_kernel<OUT_BF16, G>, tm_a, tm_b, tm_out, p, tma_store));
   return TCFP_OK;
 }
 
@@ -668,7 +682,10 @@ extern "C" int32_t tcfp_int8_gemm(const int8_t* a, int64_t ld_a, const float* s_
   // 28.1, 512: 35.8 / 28.5; 22016 x 4096, 128: 23.7 / 31.5, 256: 39.1 / 32.1; 1024 x 1024, 1024: 6.9 / 10.1.
   const int64_t rows = (N + 127) / 128, tiles = rows * ((M + 127) / 128), pair_tiles = ((N + 255) / 256) * ((M + 255) / 256);
   if (M > 64 && tiles > sm_count() && (tiles > 2 * sm_count() || 2 * pair_tiles <= sm_count()))
-    return p.out_bf16 ? launch_pair<true>(o, p, stream) : launch_pair<false>(o, p, stream);
+    // a tile's K loop hides the epilogue of the tile before from K = 2048 on; for shorter ones two groups write it out.  Measured (us,
+    // one / two groups): 8192 x 12288 x 256 106 / 82, x 1024 110 / 97; x 4096 248 / 252
+    if (p.K < 2048) return p.out_bf16 ? launch_pair<true, 2>(o, p, stream) : launch_pair<false, 2>(o, p, stream);
+    else return p.out_bf16 ? launch_pair<true, 1>(o, p, stream) : launch_pair<false, 1>(o, p, stream);
   if (M <= 16) return launch_few<16>(o, p, stream);
   if (M <= 32) return launch_few<32>(o, p, stream);
   if (M <= 64 || rows * ((M + 63) / 64) <= sm_count()) return launch_few<64>(o, p, stream);
