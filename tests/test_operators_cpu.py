@@ -97,3 +97,30 @@ def test_python_refusals():
         K.silu_mul_quantize(x, torch.zeros(2, 32))
     with pytest.raises(TypeError, match="out_dtype"):
         K.int8_matmul(x.to(torch.int8), x.to(torch.int8), torch.ones(2), torch.ones(2), out_dtype=torch.float16)
+
+
+def test_module_refusals():
+    from tcfp_b200.nn import Int8Linear, QuantizedRMSNorm, convert_to_int8
+
+    for kw in (dict(d=96, scale_block_size=64), dict(d=128, scale_block_size=48)):
+        with pytest.raises(ValueError, match="scale_block_size"):
+            QuantizedRMSNorm(**kw)
+    with pytest.raises(ValueError, match="out_dtype"):
+        Int8Linear(16, 16, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="131071"):
+        Int8Linear(131072, 1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        convert_to_int8(torch.nn.Sequential(torch.nn.Linear(16, 16)))
+    layer = Int8Linear(30, 5)
+    assert layer.weight_codes.shape == (5, 32) and set(layer.state_dict()) == {"weight_codes", "weight_scale", "bias"}
+    assert layer.to(torch.bfloat16).weight_scale.dtype == torch.float32 and layer.bias.dtype == torch.float32
+    assert Int8Linear(16, 16, bias=False).to(torch.float64).weight_scale.dtype == torch.float32
+
+
+def test_column_parallel_parts_and_packed_output():
+    from tcfp_b200.tp import ColumnParallelLinear
+
+    layer = ColumnParallelLinear(8, (32, 16), layer_factory=lambda i, o, b, **kw: torch.nn.Linear(i, o, b))
+    x = torch.randn(3, 8)
+    parts, packed = layer(x), layer(x, packed=True)
+    assert [p.shape[-1] for p in parts] == [32, 16] and torch.equal(torch.cat(parts, dim=-1), packed)
