@@ -677,15 +677,16 @@ extern "C" int32_t tcfp_int8_gemm(const int8_t* a, int64_t ld_a, const float* s_
   p.status = device_status_ptr();
   p.wide_out = N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   // Tokens a tile: all of them up to 64; beyond, 64 while that leaves no SM two tiles, else 128.  The pairs take over where
-  // tiles of 128 would not all be resident (two an SM), or would share SMs while the pairs need one tile each.  Measured (us,
-  // few / pairs): 4096 x 4096, 256 tokens 11.6 / 16.8, 512: 13.6 / 17.2, 640: 17.9 / 16.9; 12288 x 4096, 128: 16.8 / 19.3, 384: 21.1 /
-  // 28.1, 512: 35.8 / 28.5; 22016 x 4096, 128: 23.7 / 31.5, 256: 39.1 / 32.1; 1024 x 1024, 1024: 6.9 / 10.1.
+  // tiles of 128 would not all be resident (two an SM), or would share SMs while the pairs need one tile each.  Measured
+  // (us, few / pairs): 4096 x 4096, 256 tokens 11.6 / 16.8, 512: 13.6 / 17.2, 640: 17.9 / 16.9; 12288 x 4096, 128: 16.8 / 19.3,
+  // 384: 21.1 / 28.1, 512: 35.8 / 28.5; 22016 x 4096, 128: 23.7 / 31.5, 256: 39.1 / 32.1; 1024 x 1024, 1024: 6.9 / 10.1.
   const int64_t rows = (N + 127) / 128, tiles = rows * ((M + 127) / 128), pair_tiles = ((N + 255) / 256) * ((M + 255) / 256);
-  if (M > 64 && tiles > sm_count() && (tiles > 2 * sm_count() || 2 * pair_tiles <= sm_count()))
-    // a tile's K loop hides the epilogue of the tile before from K = 2048 on; for shorter ones two groups write it out.  Measured (us,
-    // one / two groups): 8192 x 12288 x 256 106 / 82, x 1024 110 / 97; x 4096 248 / 252
-    if (p.K < 2048) return p.out_bf16 ? launch_pair<true, 2>(o, p, stream) : launch_pair<false, 2>(o, p, stream);
-    else return p.out_bf16 ? launch_pair<true, 1>(o, p, stream) : launch_pair<false, 1>(o, p, stream);
+  if (M > 64 && tiles > sm_count() && (tiles > 2 * sm_count() || 2 * pair_tiles <= sm_count())) {
+    // From K = 2048 on a tile's K loop hides the epilogue of the tile before; for shorter ones two groups write it out.
+    // Measured (us, one / two groups): 8192 x 12288 x 256 106 / 82, x 1024 110 / 97, x 4096 248 / 252.
+    if (K < 2048) return p.out_bf16 ? launch_pair<true, 2>(o, p, stream) : launch_pair<false, 2>(o, p, stream);
+    return p.out_bf16 ? launch_pair<true, 1>(o, p, stream) : launch_pair<false, 1>(o, p, stream);
+  }
   if (M <= 16) return launch_few<16>(o, p, stream);
   if (M <= 32) return launch_few<32>(o, p, stream);
   if (M <= 64 || rows * ((M + 63) / 64) <= sm_count()) return launch_few<64>(o, p, stream);
