@@ -575,6 +575,10 @@ def _pitch16(t: torch.Tensor, ld: int) -> bool:
     return t.data_ptr() % 16 == 0 and (ld * t.element_size()) % 16 == 0
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, requires_grad=False) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _check_block(block_size, width: int, who: str) -> None:
     if block_size is None:
         return
@@ -587,20 +591,21 @@ def _check_block(block_size, width: int, who: str) -> None:
 def _alloc_quantized(x: torch.Tensor, rows: int, width: int, block_size, want_bf16: bool, shape) -> tuple:
     """The outputs of a row quantizer: ``(QuantizedActivation, sf or None,
     row pitch of the codes)``."""
-    deq = x.new_empty((rows, width), dtype=torch.bfloat16) if want_bf16 else None
+    dev = x.device
+    # empty_strided is the cheapest allocation there is (1.5 us of host time; empty 2.4, a slice of a padded one 1.7 more)
+    new = torch.empty_strided
+    deq = new((rows, width), (width, 1), dtype=torch.bfloat16, device=dev) if want_bf16 else None
     if block_size is not None:
-        codes = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
-        scales = x.new_empty((width // block_size, rows), dtype=torch.int8)
-        sf = _alloc_sf(rows, width, block_size, x.device)
+        codes = new((rows, width), (width, 1), dtype=torch.float8_e4m3fn, device=dev)
+        scales = new((width // block_size, rows), (rows, 1), dtype=torch.int8, device=dev)
+        sf = _alloc_sf(rows, width, block_size, dev)
         _attach_sf(scales, sf, block_size)
         pitch = width
     else:
         # the int8 product reads rows that start on 16-byte boundaries
         pitch = -(-width // 16) * 16
-        codes = x.new_empty((rows, pitch), dtype=torch.int8)
-        if pitch != width:
-            codes = codes[:, :width]
-        scales = x.new_empty(rows, dtype=torch.float32)
+        codes = new((rows, width), (pitch, 1), dtype=torch.int8, device=dev)
+        scales = new((rows,), (1,), dtype=torch.float32, device=dev)
         sf = None
     return QuantizedActivation(codes, scales, block_size, shape, x.dtype, deq), sf, pitch
 
@@ -632,8 +637,8 @@ def add_rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch
         if w.data_ptr() % 16:
             w = w.clone()
     q, sf, pitch = _alloc_quantized(x, rows, width, block_size, want_bf16, x.shape)
-    h = None if residual is None else x.new_empty(x.shape)
-    rstd = x.new_empty(rows, dtype=torch.float32)
+    h = None if residual is None else _dense_like(x)
+    rstd = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
     if rows > 0:
         _launch(x.device, _C.load().tcfp_add_rms_norm_quantize, x2d.data_ptr(), ld_x, _C.ptr(r2d), ld_r, _C.dtype_code(x2d),
                 w.data_ptr(), _C.dtype_code(w), eps, _C.ptr(h), rstd.data_ptr(), q.codes.data_ptr(), pitch,
@@ -661,8 +666,8 @@ def add_rms_norm_backward(grad: torch.Tensor, h: torch.Tensor, rstd: torch.Tenso
         return torch.empty_like(h), torch.zeros(width, dtype=torch.float32, device=h.device)
     g2d, ld_g = _rows_of(grad, who, "grad")
     d2d, ld_d = (None, 0) if grad_h is None else _rows_of(grad_h, who, "grad_h")
-    dx = h.new_empty(h.shape)
-    dw = h.new_empty(width, dtype=torch.float32)
+    dx = _dense_like(h)
+    dw = torch.empty_strided((width,), (1,), dtype=torch.float32, device=h.device)
     lib = _C.load()
     if h.device.index == torch._C._cuda_getDevice():      # the workspace goes by the device's number of SMs
         nbytes = lib.tcfp_rms_norm_backward_workspace_bytes(rows, width)
@@ -731,8 +736,8 @@ def silu_mul_backward(grad: torch.Tensor, gate: torch.Tensor, up: torch.Tensor |
         raise ValueError(f"{who}: grad must be {tuple(shape)} {gate.dtype} on {gate.device}, got {tuple(grad.shape)} "
                          f"{grad.dtype} on {grad.device}")
     d2d, ld_d = _rows_of(grad, who, "grad")
-    dg = gate.new_empty(gate.shape)
-    du = None if up is None else gate.new_empty(gate.shape)
+    dg = _dense_like(gate)
+    du = None if up is None else _dense_like(gate)
     if rows > 0:
         at = dg.data_ptr()
         ld = 2 * width if up is None else width
@@ -794,7 +799,7 @@ def int8_matmul(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale
     b_scale = _vector(b_scale, N, a.device, who, "b_scale")
     if bias is not None:
         bias = _vector(bias, N, a.device, who, "bias", (torch.float32, torch.bfloat16)).float()
-    out = a.new_empty((M, N), dtype=out_dtype)
+    out = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=a.device)
     if M > 0:
         _launch(a.device, _C.load().tcfp_int8_gemm, a.data_ptr(), ld_a, a_scale.data_ptr(), b.data_ptr(), ld_b,
                 b_scale.data_ptr(), _C.ptr(bias), out.data_ptr(), code, M, N, K)
