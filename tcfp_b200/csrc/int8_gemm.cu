@@ -247,7 +247,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(mapa(bar_tempty + 8 * buf, 0));
         }
-        // a piece may be rewritten once the store that last used it has read it
+        // a piece may be rewritten once the store that last used it has read it: with one group that is the piece before last,
+        // with two groups the last one
         if (!OUT_BF16 || (g & 1) == 0) {
           if (issuer) {
             if constexpr (G == 1) bulk_wait_read1();
@@ -278,8 +279,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         if (tma_store) {
           fence_async_smem();
           epi_sync(id);
-          if (issuer && nst < p.N && row0 < p.M) {
-            tma_store_2d(&tm_out, smem_u32(piece), nst, row0);
+          if (issuer) {
+            // a piece outside the output commits an empty group, so that the wait above counts pieces
+            if (nst < p.N && row0 < p.M) tma_store_2d(&tm_out, smem_u32(piece), nst, row0);
             bulk_commit();
           }
         } else {
