@@ -342,7 +342,6 @@ dual_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
     constexpr int kPieceCols = OUT_BF16 ? 64 : 32;     // output columns per 128-byte staging row
     int buf = 0;
     uint32_t buf_phase = 0;
-    int pending = 0;          // TMA stores in flight (issuer only)
     int sbuf = 0;             // staging buffer for the next store
     bool live = true;
     for (int tile = pair; live && tile < num_tiles; tile += num_pairs) {
@@ -378,10 +377,10 @@ dual_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
           for (int i = 0; i < 32; ++i)
             if (n0 + i < p.N) o[i] += __ldg(p.bias + n0 + i);
         }
-        // a staging buffer may be rewritten once the store issued two pieces ago has read it
+        // a staging buffer may be rewritten once the store issued two pieces ago has read it: every piece commits a group
         const bool new_row = OUT_BF16 ? ((g & 1) == 0) : true;
         if (new_row) {
-          if (issuer && pending >= 2) { bulk_wait_read1(); pending = 1; }
+          if (issuer) bulk_wait_read1();
           epi_bar_sync();
         }
         uint8_t* piece = staging + sbuf * kPieceBytes + r_local * 128;
@@ -413,11 +412,9 @@ dual_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_con
           epi_bar_sync();
           if (issuer) {
             const int nst = OUT_BF16 ? (nb * tile_n + (g >> 1) * kPieceCols) : n0;
-            if (nst < p.N && row0 < p.M) {
-              tma_store_2d(&tm_out, smem_u32(staging + sbuf * kPieceBytes), nst, row0);
-              bulk_commit();
-              ++pending;
-            }
+            // a piece outside the output commits an empty group, so that the wait above counts pieces
+            if (nst < p.N && row0 < p.M) tma_store_2d(&tm_out, smem_u32(staging + sbuf * kPieceBytes), nst, row0);
+            bulk_commit();
           }
           sbuf ^= 1;
         }
