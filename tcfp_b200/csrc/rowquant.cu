@@ -727,6 +727,7 @@ int launch_row(const RowParams& p, cudaStream_t stream) {
     // even shares of up to 128 threads, in multiples of four scale blocks (a word of packed scale factors)
     const int grain = p.block == 128 ? 64 : 32;
     col_blocks = (units + 127) / 128;
+    if (col_blocks > 65535) col_blocks = (units + 255) / 256;      // what gridDim.y can hold: the widest rows take 256 threads
     threads = ((units + col_blocks - 1) / col_blocks + grain - 1) / grain * grain;
   } else {
     nc = units <= 64 ? 1 : units <= 1024 ? 2 : units <= 4096 ? 4 : 0;
