@@ -27,11 +27,14 @@ scale would cost two dependent all-reduce(max) rounds per layer per step.
 """
 from __future__ import annotations
 
+import copy
 from typing import Callable
 
 import torch
 import torch.distributed as dist
 import torch.nn as nn
+
+from .kernels import QuantizedActivation
 
 
 _COLLECTIVES_ENABLED = True
@@ -381,16 +384,36 @@ class ColumnParallelLinear(nn.Module):
             self.inner._hooks = LayerHooks(sp=SequenceParallelIO(group), reserve_sms=comm_sms)
 
     def forward(self, x, packed: bool = False):
-        """``x``: a tensor, or the ``QuantizedActivation`` the inner layer takes.
-        ``packed=True``: the parts' local outputs as one tensor."""
+        """``x``: a tensor, or the ``QuantizedActivation`` the inner layer takes
+        (over several ranks of a sequence-parallel group: a ``TCFPLinear``,
+        which gathers the codes).  ``packed=True``: the parts' local outputs as
+        one tensor."""
         if self.sequence_parallel and not self._sp_fused:
-            x = _GatherFromSequenceParallel.apply(x, self.group)
+            x = self._gathered(x)
         if self.reduce_input_grad and not self._overlap:
-            x = _CopyToParallel.apply(x, self.group)
+            x = self._with_reduced_grad(x)
         y = self.inner(x)
         if self.fused and not packed:
             return torch.split(y, self.local_sizes, dim=-1)
         return y
+
+    def _gathered(self, x):
+        if not isinstance(x, QuantizedActivation):
+            return _GatherFromSequenceParallel.apply(x, self.group)
+        if dist.is_initialized() and dist.get_world_size(self.group) > 1:
+            raise TypeError(f"a sequence-parallel {type(self.inner).__name__} takes a tensor: only a TCFPLinear gathers the codes "
+                            "of a quantized activation")
+        return x
+
+    def _with_reduced_grad(self, x):
+        if not isinstance(x, QuantizedActivation):
+            return _CopyToParallel.apply(x, self.group)
+        if x._handle is None:
+            return x
+        # the codes as they are, the gradient through an all-reduce; other layers that take x keep their own path to it
+        x = copy.copy(x)
+        x._handle = _CopyToParallel.apply(x._handle, self.group)
+        return x
 
 
 def copy_to_parallel(x: torch.Tensor, group=None) -> torch.Tensor:
