@@ -798,15 +798,32 @@ class Int8Linear(nn.Module):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, *, out_dtype: torch.dtype = torch.float32,
                  device=None):
         super().__init__()
-        if out_dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
-        if not 1 <= in_features <= 131071:
-            raise ValueError(f"in_features ({in_features}) must be in [1, 131071]: the integer sums have 32 bits")
+        self._check_sizes(in_features, out_dtype)
         self.in_features, self.out_features, self.out_dtype = in_features, out_features, out_dtype
         # rows padded to 16 bytes, as the product reads them
         self.register_buffer("weight_codes", torch.zeros(out_features, -(-in_features // 16) * 16, dtype=torch.int8, device=device))
         self.register_buffer("weight_scale", torch.ones(out_features, dtype=torch.float32, device=device))
         self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32, device=device) if bias else None)
+
+    @staticmethod
+    def _check_sizes(in_features: int, out_dtype: torch.dtype) -> None:
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("out_dtype must be torch.float32 or torch.bfloat16")
+        if not 1 <= in_features <= 131071:
+            raise ValueError(f"in_features ({in_features}) must be in [1, 131071]: the integer sums have 32 bits")
+
+    @classmethod
+    def _source(cls, linear: nn.Module, out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.dtype]:
+        """The weight of a layer and the output type of its int8 form; raises
+        where there is none."""
+        w = linear.weight.detach()
+        if out_dtype is None:
+            out_dtype = getattr(linear, "out_dtype", w.dtype)
+        cls._check_sizes(w.shape[1], out_dtype)
+        if not w.is_cuda:
+            raise RuntimeError(f"Int8Linear: tcfp_b200 runs on CUDA (sm_100) tensors only, got a {w.device} weight")
+        _C.dtype_code(w)
+        return w, out_dtype
 
     def _apply(self, fn, *args, **kw):
         # scale and bias stay FP32 when a model is cast to another type
@@ -823,9 +840,7 @@ class Int8Linear(nn.Module):
         """From an ``nn.Linear`` or ``TCFPLinear`` on the GPU; the output type is
         the layer's own unless given (``TCFPLinear.out_dtype``, else the
         weight's)."""
-        w = linear.weight.detach()
-        if out_dtype is None:
-            out_dtype = getattr(linear, "out_dtype", w.dtype)
+        w, out_dtype = cls._source(linear, out_dtype)
         new = cls(w.shape[1], w.shape[0], linear.bias is not None, out_dtype=out_dtype, device=w.device)
         q = int8_quantize_rows(w)
         new.weight_codes[:, :w.shape[1]].copy_(q.codes)
@@ -854,21 +869,30 @@ class Int8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
+def _int8_candidates(model: nn.Module, skip_patterns: tuple[str, ...]):
+    """(parent, name, layer) of what :func:`convert_to_int8` replaces."""
+    for name, module in model.named_children():
+        yield from _int8_candidates(module, skip_patterns)
+        if any(pat in name for pat in skip_patterns) or not isinstance(module, (nn.Linear, TCFPLinear)):
+            continue
+        if not isinstance(module, nn.modules.linear.NonDynamicallyQuantizableLinear):
+            yield model, name, module
+
+
 def convert_to_int8(model: nn.Module, skip_patterns: tuple[str, ...] = ("head",)) -> nn.Module:
     """Swaps the ``nn.Linear`` and ``TCFPLinear`` children of a model on the GPU
     for ``Int8Linear`` in place, with the traversal and ``skip_patterns`` of
     :func:`convert_to_tcfp`.  A layer that communicates in its forward pass
     (row- or sequence-parallel over more than one rank) is refused; the output
     projection of ``nn.MultiheadAttention``, whose weight that module reads
-    itself, stays as it is."""
-    for name, module in list(model.named_children()):
-        convert_to_int8(module, skip_patterns)
-        if any(pat in name for pat in skip_patterns) or not isinstance(module, (nn.Linear, TCFPLinear)):
-            continue
-        if isinstance(module, nn.modules.linear.NonDynamicallyQuantizableLinear):
-            continue
+    itself, stays as it is.  A model with a refused layer is left as it was."""
+    found = list(_int8_candidates(model, skip_patterns))
+    for _, name, module in found:
         hooks = getattr(module, "_hooks", None)
         if hooks is not None and (hooks.out_hook is not None or hooks.sp is not None or hooks.sp_out is not None):
             raise ValueError(f"{name}: a layer that reduces or gathers over ranks in its forward pass has no int8 form")
-        setattr(model, name, Int8Linear.from_linear(module))
+        Int8Linear._source(module)
+    while found:           # a replaced layer is let go before the next one is built
+        parent, name, module = found.pop(0)
+        setattr(parent, name, Int8Linear.from_linear(module))
     return model
