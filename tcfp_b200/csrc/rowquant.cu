@@ -155,13 +155,16 @@ __device__ __forceinline__ float row_reduce(float v, float* slots) {
 
 // ---- the operators ------------------------------------------------------------------
 // sigma(g) = 1 / (1 + 2^(-g log2 e)) by the approximate instructions that flush what is below 2^-126: good to about |g| + 8
-// units of 2^-24 (the product's rounding becomes the exponent's error), with the limits 0 and 1 for large |g|.
+// units of 2^-24 (the product's rounding becomes the exponent's error), with the limits 0 and 1 for large |g|.  For outputs of
+// 8 or 16 bits, whose rounding is a thousand times that.
 __device__ __forceinline__ float sigmoid(float g) {
   float t, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(g * -1.44269504f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + t));
   return r;
 }
+// The same good to 6 units of 2^-24 for every g, for outputs that stay in 32 bits.
+__device__ __forceinline__ float sigmoid_f32(float g) { return __frcp_rn(1.f + expf(-g)); }
 __device__ __forceinline__ float gated(float g, float u) { return g * sigmoid(g) * u; }
 
 // eight values of the one or two inputs of a row
@@ -664,7 +667,8 @@ struct GateBwdParams {
   int width;
 };
 
-// sigma = 1/(1+e^-g): dgate = dy * u * sigma * (1 + g (1 - sigma)), dup = dy * g * sigma
+// sigma = 1/(1+e^-g): dgate = dy * u * sigma * (1 + g (1 - sigma)), dup = dy * g * sigma.  Bound by memory in either type:
+// FP32 8192 x 11008 268 us with the longer sigma, 273 us with the short one; bf16 16384 x 11008 273 us.
 template <bool BF16, bool VEC>
 __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
   let_next_start();
@@ -678,7 +682,7 @@ __global__ void silu_mul_backward_kernel(const GateBwdParams p) {
   load8<BF16, VEC>(u, p.up, row * p.ld_up + i0, p.width - i0, step);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float sig = sigmoid(g[j]);
+    const float sig = BF16 ? sigmoid(g[j]) : sigmoid_f32(g[j]);
     const float ds = d[j] * sig;
     const float dg = ds * u[j] * fmaf(g[j], 1.f - sig, 1.f);
     u[j] = ds * g[j];
