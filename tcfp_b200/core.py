@@ -225,7 +225,8 @@ class ErrorFeedbackState:
         """The buffer for ``name``: FP32, zero on first use or after a shape change."""
         buf = self._buffers.get(name)
         if buf is None or buf.shape != like.shape:
-            buf = torch.zeros_like(like, dtype=torch.float32)
+            with torch.inference_mode(False):       # also updated in place by a training step after an inference call
+                buf = torch.zeros_like(like, dtype=torch.float32)
             self._buffers[name] = buf
         return buf
 

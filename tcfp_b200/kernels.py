@@ -71,7 +71,10 @@ def packed_scale_rows(sf: torch.Tensor, r0: int, r1: int, K: int, block_size: in
 
 def _attach_sf(exps: torch.Tensor, sf: torch.Tensor, block_size: int) -> None:
     # the packed copy is only valid for the bytes it was packed from: remember the plane's
-    # version counter and address so that an in-place edit or a re-bound storage repacks
+    # version counter and address so that an in-place edit or a re-bound storage repacks.  An inference tensor has no
+    # counter: its plane is packed again where it is used
+    if exps.is_inference():
+        return
     exps._tcfp_sf = (sf, exps._version, exps.data_ptr(), block_size)
 
 

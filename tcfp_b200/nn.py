@@ -132,9 +132,12 @@ def _cached_quantize(cache: dict | None, w: torch.Tensor, error_buf, update_ef: 
     layer, keyed on the weight's and the buffer's version counters and
     addresses.  Not used for the stochastic residual (fresh randoms per
     forward), for a forward that updates the error buffer, or while a CUDA
-    graph is being captured (a replayed step must quantize the weight it finds)."""
+    graph is being captured (a replayed step must quantize the weight it finds).
+    In inference mode the kept tensors are ordinary ones all the same: they are
+    used again outside of it."""
     reusable = (cache is not None and not srr and (error_buf is None or not update_ef)
-                and not torch.cuda.is_current_stream_capturing())
+                and not torch.cuda.is_current_stream_capturing()
+                and not w.is_inference() and (error_buf is None or not error_buf.is_inference()))
     if not reusable:
         if cache is not None:
             cache.clear()
@@ -143,7 +146,8 @@ def _cached_quantize(cache: dict | None, w: torch.Tensor, error_buf, update_ef: 
            None if error_buf is None else (error_buf.data_ptr(), error_buf._version))
     if cache.get("key") == key:
         return cache["value"]
-    value = quantize()
+    with torch.inference_mode(False), torch.no_grad():
+        value = quantize()
     cache["key"], cache["value"] = key, value
     return value
 
