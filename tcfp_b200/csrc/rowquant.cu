@@ -708,8 +708,10 @@ int block_shift(int block) { return block == 128 ? 7 : block == 64 ? 6 : 5; }
 // 215 us; 8 rows a block 149 us, 16 rows 155 us, 1 row 230 us (nothing ahead, and the exponents leave as single bytes).
 // Narrower rows want more of them: 16384 x 1024 27 us with 8 rows, 23 us with 32.  A row of more than 8192 values takes 32 a
 // thread and no load ahead (registers); up to 12288 three blocks share an SM: gate 16384 x 11008 to int8 153 us (5.9 TB/s),
-// two blocks 195 us.  The gated block form has no row statistic: 128 threads x 8 values walk 16 rows of 1024 columns,
-// 16384 x 11008 155 us (5.8 TB/s), with bf16 values 208 us (6.1 TB/s); 256 threads 175 and 234 us (before the shorter sigmoid).
+// two blocks 195 us.  That form keeps its values in 56 registers; the norm, FP32 and single-value forms spill 8 to 276 bytes a
+// thread there (norm 16384 x 11008 to int8 299 us, 4.2 TB/s) and were not timed with two blocks.  The gated block form has no
+// row statistic: 128 threads x 8 values walk 16 rows of 1024 columns, 16384 x 11008 155 us (5.8 TB/s), with bf16 values 208 us
+// (6.1 TB/s); 256 threads 175 and 234 us (before the shorter sigmoid).
 // Rows off 16-byte boundaries take single values and are bound by their instructions: 16384 x 1001 FP32 norm 49 us (3.7 TB/s).
 template <int OP, bool BF16, bool VEC, bool BLOCK>
 int launch_row(const RowParams& p, cudaStream_t stream) {

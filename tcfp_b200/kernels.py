@@ -502,7 +502,11 @@ class QuantizedActivation:
     :func:`block_quantize_fp8` returns.  ``block_size`` ``None``: int8 codes
     and one float scale for each row; the rows start on 16-byte boundaries.
     ``bf16`` holds the values the codes stand for if they were asked for.
-    ``dtype`` is the type of the tensor the activation was computed from."""
+    ``dtype`` is the type of the tensor the activation was computed from.
+
+    It is neither a tensor nor a pytree node: a full backward hook on a module
+    that takes one is given ``None`` for it, and a wrapper that looks for tensors
+    in a module's inputs or outputs does not see the path of its gradient."""
 
     def __init__(self, codes, scales, block_size, shape, dtype, bf16=None):
         self.codes, self.scales, self.block_size = codes, scales, block_size
