@@ -562,6 +562,18 @@ int allow_smem(Kernel kern, int bytes, bool (&done)[64]) {
 constexpr int kSmemLimit = 232448;       // of a block
 constexpr int kSmemSm = 233472;          // of an SM; 1 KB of it goes with every block
 
+// A block of the few-token kernel lets the next kernel's blocks in before it has its columns of TMEM, and those wait for it with
+// theirs: whatever shares an SM has to fit into its 512 columns together.  A pair's block, which takes all of them, never fits
+// beside a few-token block's shared memory, and as many of those as do fit stay below 512: none has more columns for its shared
+// memory than the 128-token form, three of which have 384.
+constexpr int kTmemColumns = 512;
+static_assert(kPairSmem + 1024 + Few<16>::smem(Few<16>::kMinStages) + 1024 > kSmemSm, "a pair's block beside a few-token block");
+template <int NT>
+constexpr bool few_fit_tmem() {
+  return kSmemSm / (Few<NT>::smem(Few<NT>::kMinStages) + 1024) * (int)Few<NT>::kTmemCols <= kTmemColumns;
+}
+static_assert(few_fit_tmem<16>() && few_fit_tmem<32>() && few_fit_tmem<64>() && few_fit_tmem<128>(), "few-token blocks of an SM");
+
 struct Operands {
   const int8_t *a, *b;
   int64_t lda, ldb;
