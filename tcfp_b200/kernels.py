@@ -432,6 +432,10 @@ def retarget_block_weights(w_hi_fp8, w_lo_fp8, w_hi_scales, w_lo_scales, block_s
     kept on ``w_hi_fp8`` and reused while none of the four inputs changes, so
     gradient-accumulation micro-batches pay for it once."""
     D_out, D_in = w_hi_fp8.shape
+    if any(t is not None and t.is_inference() for t in (w_hi_fp8, w_hi_scales, w_lo_fp8, w_lo_scales)):
+        # no version counter tells of a change: nothing is kept
+        hi_t, lo_t, t_hi, t_lo = block_retarget(w_hi_fp8, w_lo_fp8, w_hi_scales, w_lo_scales, block_size)
+        return hi_t, lo_t, pack_block_scales(t_hi, block_size), None if t_lo is None else pack_block_scales(t_lo, block_size)
     key = (w_hi_fp8._version, w_hi_scales._version, w_hi_scales.data_ptr(), block_size,
            None if w_lo_fp8 is None else (w_lo_fp8.data_ptr(), w_lo_fp8._version, w_lo_scales._version))
     cached = getattr(w_hi_fp8, "_tcfp_dx", None)

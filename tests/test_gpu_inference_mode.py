@@ -49,3 +49,28 @@ def test_an_edited_plane_is_packed_again():
         one = K.block_scaled_gemm(a, b, ea, eb, 64)
         ea += 1
         assert torch.equal(K.block_scaled_gemm(a, b, ea, eb, 64), 2 * one)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+def test_input_gradient_product(residual):
+    """The weight re-targeted for the input gradient is formed again where its operands have no version counter."""
+    from tcfp_b200 import kernels as K
+
+    w, g = rand(54, 192, 128), rand(55, 70, 192, dtype=torch.bfloat16)
+
+    def product(edit):
+        hi, lo, eh, el = K.fused_dual_quantize_fp8(w, 64, torch.zeros_like(w))
+        if not residual:
+            lo = el = None
+        gq, eg = K.block_quantize_fp8(g, 64, torch.float8_e5m2)
+        one = K.fused_block_scaled_backward_dx(gq, hi, lo, eg, eh, el, 64)
+        if edit:
+            eh += 1
+            if residual:
+                el += 1
+        return one, K.fused_block_scaled_backward_dx(gq, hi, lo, eg, eh, el, 64)
+
+    want, _ = product(False)
+    with torch.inference_mode():
+        one, two = product(True)
+    assert torch.equal(one, want) and torch.equal(two, 2 * want)
